@@ -9,10 +9,16 @@ namespace moodist {
 
 using BackendClass = pybind11::class_<MoodistBackend, c10d::Backend, c10::intrusive_ptr<MoodistBackend>>;
 
-// ops.cc: GEMM and fused ops
+// ops.cc: GEMM and fused ops; the status word that kernels outside a process group report to (device address), and the
+// check that an earlier one of them did not give up waiting
+uint32_t* kernel_status(int device);
+void check_kernel_status(int device);
 void bind_ops(pybind11::module_& m, BackendClass& backend);
 void bind_fused(pybind11::module_& m);
 void bind_train_ops(pybind11::module_& m);
+
+// decoder_glue.cc: layer norm, rotary positions, distillation loss, gated projection
+void bind_decoder_ops(pybind11::module_& m);
 
 // store_glue.cc: TcpStore
 void bind_store(pybind11::module_& m);
@@ -30,6 +36,7 @@ inline void bind_extras(pybind11::module_& m, BackendClass& backend) {
   bind_ops(m, backend);
   bind_fused(m);
   bind_train_ops(m);
+  bind_decoder_ops(m);
   bind_store(m);
   bind_queue(m, backend);
   bind_custom_op(m, backend);

@@ -66,6 +66,9 @@ at::Tensor gemm(const at::Tensor& a, const at::Tensor& b, bool trans_a, bool tra
 
 }  // namespace
 
+uint32_t* kernel_status(int device) { return status_word(device).dev; }
+void check_kernel_status(int device) { check_status(device); }
+
 void bind_ops(pybind11::module_& m, BackendClass& backend) {
   m.def("gemm", &gemm, pybind11::arg("a"), pybind11::arg("b"), pybind11::arg("trans_a") = false,
         pybind11::arg("trans_b") = false, pybind11::arg("out") = pybind11::none(), pybind11::arg("out_fp32") = false,

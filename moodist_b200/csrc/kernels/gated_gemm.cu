@@ -1,0 +1,128 @@
+// Host side of the gated projection and the elementwise half of its backward pass.
+#include "gated_tcgen05.cuh"
+#include "kernels_api.h"
+#include "vec_io.cuh"
+
+#define MB_STREAM(s) reinterpret_cast<cudaStream_t>(s)
+
+namespace mb {
+namespace gemm {
+int make_tmap_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
+}
+namespace gated {
+
+constexpr int kMaxDevices = 64;
+
+__global__ void __launch_bounds__(kNumThreads, 1)
+    gated_pair_kernel(const __grid_constant__ GatedParams p, const __grid_constant__ CUtensorMap tmap_x,
+                      const __grid_constant__ CUtensorMap tmap_w) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  gated_pair_body(p, &tmap_x, &tmap_w, smem_raw);
+}
+
+static int launch_pair(GatedParams& p, const CUtensorMap& tx, const CUtensorMap& tw, int device, cudaStream_t stream) {
+  static int max_clusters[kMaxDevices];  // 0: not asked yet
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kNumThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (max_clusters[device] == 0) {
+    int sms = 0, n = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaFuncSetAttribute(gated_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes) != cudaSuccess)
+      return MB_ERR_LAUNCH;
+    cfg.gridDim = dim3(sms & ~1, 1, 1);
+    if (cudaOccupancyMaxActiveClusters(&n, gated_pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = sms / 2;
+    }
+    max_clusters[device] = n < sms / 2 ? n : sms / 2;
+  }
+  const int tiles = p.tiles_m * p.tiles_n;
+  p.num_ctas = 2 * (tiles < max_clusters[device] ? tiles : max_clusters[device]);
+  cfg.gridDim = dim3(p.num_ctas, 1, 1);
+  return cudaLaunchKernelEx(&cfg, gated_pair_kernel, p, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+}
+
+// dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F], bound by their bytes.
+// The results are rounded to bf16 because the two matrix products that follow take bf16 operands.
+template <int kAct>
+__global__ void __launch_bounds__(256)
+    gated_bwd_kernel(const __nv_bfloat16* __restrict__ gu, const __nv_bfloat16* __restrict__ dh, __nv_bfloat16* __restrict__ dgu,
+                     int64_t T, int F, int64_t ldgu, int64_t lddh, int64_t lddgu) {
+  const int vecs = F / 8;
+  const int64_t total = T * vecs;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / vecs;
+    const int j = (int)(i % vecs) * 8;
+    float g[8], u[8], d[8];
+    load_vec<__nv_bfloat16, 8>(gu + t * ldgu + j, g);
+    load_vec<__nv_bfloat16, 8>(gu + t * ldgu + F + j, u);
+    load_vec<__nv_bfloat16, 8>(dh + t * lddh + j, d);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float2 a = activate_slope(kAct, g[k]);
+      g[k] = d[k] * u[k] * a.y;
+      u[k] = d[k] * a.x;
+    }
+    store_vec<__nv_bfloat16, 8>(dgu + t * lddgu + j, g);
+    store_vec<__nv_bfloat16, 8>(dgu + t * lddgu + F + j, u);
+  }
+}
+
+}  // namespace gated
+}  // namespace mb
+
+using namespace mb;
+using namespace mb::gated;
+
+extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, int64_t T, int F, int K, int64_t ldx, int64_t ldw,
+                                 int64_t ldh, int64_t ldgu, int act, uint32_t* status, uint64_t wait_ns, void* stream) {
+  if (T <= 0) return MB_OK;
+  if (F <= 0 || K <= 0 || T > (1 << 30) || F > (1 << 29) || act < 0 || act > 2) return MB_ERR_ARG;
+  if (F % 8 || K % 8 || ldx % 8 || ldw % 8 || ldh % 8 || ldgu % 8) return MB_ERR_ALIGN;
+  if (!is_aligned(x, 16) || !is_aligned(w, 16) || !is_aligned(h, 16) || !is_aligned(gu, 16)) return MB_ERR_ALIGN;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return MB_ERR_DRIVER;
+  CUtensorMap tx, tw;
+  int rc = gemm::make_tmap_bf16(&tx, x, T, K, ldx, BM);
+  if (rc) return rc;
+  rc = gemm::make_tmap_bf16(&tw, w, 2 * (uint64_t)F, K, ldw, kHCols);
+  if (rc) return rc;
+  GatedParams p{};
+  p.T = (int)T;
+  p.F = F;
+  p.K = K;
+  p.h = (__nv_bfloat16*)h;
+  p.ldh = ldh;
+  p.gu = (__nv_bfloat16*)gu;
+  p.ldgu = ldgu;
+  p.act = act;
+  p.tiles_m = (int)((T + kPairBM - 1) / kPairBM);
+  p.tiles_n = (F + kHCols - 1) / kHCols;
+  p.group_m = 4;
+  p.status = status;
+  p.wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
+  return launch_pair(p, tx, tw, device, MB_STREAM(stream));
+}
+
+extern "C" int mb_gated_bwd_bf16(const void* gu, const void* dh, void* dgu, int64_t T, int F, int64_t ldgu, int64_t lddh,
+                                 int64_t lddgu, int act, void* stream) {
+  if (T <= 0) return MB_OK;
+  if (F <= 0 || act < 0 || act > 2) return MB_ERR_ARG;
+  if (F % 8 || ldgu % 8 || lddh % 8 || lddgu % 8 || !is_aligned(gu, 16) || !is_aligned(dh, 16) || !is_aligned(dgu, 16))
+    return MB_ERR_ALIGN;
+  int64_t grid = (T * (F / 8) + 255) / 256;
+  if (grid > 148 * 16) grid = 148 * 16;
+  auto k = act == kSilu ? gated_bwd_kernel<kSilu> : act == kGelu ? gated_bwd_kernel<kGelu> : gated_bwd_kernel<kGeluTanh>;
+  k<<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((const __nv_bfloat16*)gu, (const __nv_bfloat16*)dh, (__nv_bfloat16*)dgu, T, F,
+                                                   ldgu, lddh, lddgu);
+  return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+}

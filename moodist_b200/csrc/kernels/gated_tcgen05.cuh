@@ -1,0 +1,274 @@
+// Gated projection on tcgen05: h = act(x Wg^T) * (x Wu^T), both products, the activation and their product in one kernel.
+//
+//   x [T, K], W [2F, K] (gate rows [0, F), up rows [F, 2F)), h [T, F], all bf16, accumulation fp32
+//
+// A cluster of two CTAs computes 256 rows x 128 columns of h as one 256 x 256 tile of tcgen05.mma.cta_group::2: columns
+// [0, 128) of the accumulator are gate columns, [128, 256) the up columns of the same h. The even CTA loads the gate rows of W
+// and the odd one the up rows, so each still brings 128 rows of x and 128 rows of W per 64-wide step, as in the plain
+// product, and a thread of the epilogue finds both factors of an h in its own TMEM lane. The activation runs on the fp32
+// accumulators: h is rounded once. With `gu` the two projections are written too (bf16, for the backward pass: 16 bits are
+// what the unfused layer keeps, and 32 would double the largest activation of a block).
+//
+// Bound by the tensor cores: 4 T F K flops. Against product + activation kernels it saves the write and read of [T, 2F]
+// (inference) or the read (training).
+#pragma once
+
+#include "gemm_pair_tcgen05.cuh"
+
+namespace mb {
+namespace gated {
+
+using namespace gemm;
+
+enum Act : int { kSilu = 0, kGelu = 1, kGeluTanh = 2 };
+
+enum GatedStatus : uint32_t {
+  kTimeoutGatedProducer = 0x121,
+  kTimeoutGatedMma = 0x122,
+  kTimeoutGatedEpilogue = 0x123,
+};
+
+constexpr int kHCols = BN / 2;  // h columns of a tile
+
+struct GatedParams {
+  int T, F, K;
+  __nv_bfloat16* h;
+  int64_t ldh;
+  __nv_bfloat16* gu;  // [T, 2F] or null
+  int64_t ldgu;
+  int act;
+  int tiles_m, tiles_n, group_m;
+  int num_ctas;
+  uint32_t* status;
+  uint64_t wait_ns;
+};
+
+// act(g); the logistic form of the tanh approximation and erfc keep the relative accuracy of the left tail
+__device__ __forceinline__ float activate(int act, float g) {
+  if (act == kSilu) return g / (1.f + __expf(-g));
+  if (act == kGelu) return g * 0.5f * erfcf(-g * 0.70710678f);
+  const float y2 = 1.5957691216f * (g + 0.044715f * g * g * g);
+  return g / (1.f + __expf(-y2));
+}
+// act(g) and its derivative
+__device__ __forceinline__ float2 activate_slope(int act, float g) {
+  if (act == kSilu) {
+    const float s = 1.f / (1.f + __expf(-g));
+    return make_float2(g * s, s * (1.f + g * (1.f - s)));
+  }
+  if (act == kGelu) {
+    const float c = 0.5f * erfcf(-g * 0.70710678f);
+    return make_float2(g * c, c + g * __expf(-0.5f * g * g) * 0.39894228f);
+  }
+  const float y2 = 1.5957691216f * (g + 0.044715f * g * g * g);
+  const float s = 1.f / (1.f + __expf(-y2));
+  return make_float2(g * s, s + g * s * (1.f - s) * 1.5957691216f * (1.f + 0.134145f * g * g));
+}
+
+__device__ __forceinline__ void gated_report(const GatedParams& p, uint32_t code) {
+  volatile uint32_t* s = p.status;
+  if (s && *s == 0) *s = code;
+}
+
+// tile index -> (m, n), grouped so that CTAs running together share panels of x and W in L2
+__device__ __forceinline__ void gated_tile(const GatedParams& p, int t, int& tm, int& tn) {
+  const int per_group = p.group_m * p.tiles_n;
+  const int g = t / per_group, first_m = g * p.group_m;
+  const int gsz = min(p.group_m, p.tiles_m - first_m);
+  const int r = t - g * per_group;
+  tm = first_m + r % gsz;
+  tn = r / gsz;
+}
+
+// 32 values of a lane's row -> its line of the warp's patch, half `h` of 64 columns
+__device__ __forceinline__ void patch_put(uint8_t* patch, int lane, int h, const float* v) {
+  uint4* dst = reinterpret_cast<uint4*>(patch + lane * kEpiRowBytes + h * 64);
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    dst[g] = make_uint4(pack_bf16x2(v[g * 8], v[g * 8 + 1]), pack_bf16x2(v[g * 8 + 2], v[g * 8 + 3]),
+                        pack_bf16x2(v[g * 8 + 4], v[g * 8 + 5]), pack_bf16x2(v[g * 8 + 6], v[g * 8 + 7]));
+}
+// the patch's 32 rows x 64 columns -> global memory as 128-byte lines
+__device__ __forceinline__ void patch_store(const uint8_t* patch, int lane, __nv_bfloat16* base, int64_t ld, int rows, int cols) {
+  __syncwarp();
+  const int col = (lane & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rr = i * 4 + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(patch + rr * kEpiRowBytes + (lane & 7) * 16);
+    if (rr < rows && col < cols) *reinterpret_cast<uint4*>(base + (int64_t)rr * ld + col) = v;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUtensorMap* tmap_x, const CUtensorMap* tmap_w,
+                                                uint8_t* smem_raw) {
+  uint32_t raw = smem_u32(smem_raw);
+  uint8_t* tiles = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kPairStages * kPairStageBytes);
+  uint64_t* full = bars;                        // [kPairStages]  used in the leader
+  uint64_t* empty = bars + kPairStages;         // [kPairStages]  one per CTA
+  uint64_t* acc_full = bars + 2 * kPairStages;  // [2]            one per CTA
+  uint64_t* acc_empty = acc_full + 2;           // [2]            used in the leader
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile uint32_t* abort_flag = tmem_base_slot + 1;
+  uint8_t* epi_patch = reinterpret_cast<uint8_t*>(bars) + 256;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta_rank = (int)cluster_ctarank();  // 0 = leader
+  const int num_tiles = p.tiles_m * p.tiles_n;
+  const int kblocks = (p.K + BK - 1) / BK;
+  const int pair = blockIdx.x >> 1, stride = p.num_ctas >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 8);  // 4 epilogue warps in each of the two CTAs
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(tmap_x);
+    tma_prefetch_desc(tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_base_slot, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  body_sync();
+  cluster_sync_all();  // the peer's barriers are initialised before anything signals them
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_base_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += stride) {
+        int tm, tn;
+        gated_tile(p, t, tm, tn);
+        const int row_x = tm * kPairBM + cta_rank * BM;
+        const int row_w = tn * kHCols + cta_rank * p.F;  // gate rows in the leader, up rows in its peer
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % kPairStages;
+          if (!mbar_wait(&empty[s], ((it / kPairStages) & 1) ^ 1, p.wait_ns)) {
+            gated_report(p, kTimeoutGatedProducer);
+            ok = false;
+            break;
+          }
+          uint8_t* sa = tiles + s * kPairStageBytes;
+          if (cta_rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStageBytes);
+          const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+          tma_load_2d_pair(sa, tmap_x, bar, kb * BK, row_x);
+          tma_load_2d_pair(sa + kATileBytes, tmap_w, bar, kb * BK, row_w);
+        }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && cta_rank == 0) {
+      constexpr uint32_t idesc = make_idesc_f16(true, false, false, kPairBM, BN);
+      uint32_t it = 0, local_tile = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += stride, ++local_tile) {
+        const uint32_t acc = local_tile & 1;
+        if (!mbar_wait(&acc_empty[acc], ((local_tile >> 1) & 1) ^ 1, p.wait_ns)) {
+          gated_report(p, kTimeoutGatedMma);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + acc * kAccCols;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % kPairStages;
+          if (!mbar_wait(&full[s], (it / kPairStages) & 1, p.wait_ns)) {
+            gated_report(p, kTimeoutGatedMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t sa = smem_u32(tiles + s * kPairStageBytes), sb = sa + kATileBytes;
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            tc_mma_f16_pair(d_tmem, make_smem_desc(sa + k * 32, 0, 1024), make_smem_desc(sb + k * 32, 0, 1024), idesc, (kb | k) != 0);
+          tc_commit_pair(&empty[s], 0x3);
+        }
+        if (ok) tc_commit_pair(&acc_full[acc], 0x3);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    const int q = warp & 3;  // TMEM lane quarter this warp may read
+    uint8_t* patch = epi_patch + (warp - 2) * kEpiPatchBytes;
+    uint32_t local_tile = 0;
+    bool ok = true;
+    for (int t = pair; t < num_tiles; t += stride, ++local_tile) {
+      int tm, tn;
+      gated_tile(p, t, tm, tn);
+      const uint32_t acc = local_tile & 1;
+      if (!mbar_wait(&acc_full[acc], (local_tile >> 1) & 1, p.wait_ns)) {
+        if (lane == 0) gated_report(p, kTimeoutGatedEpilogue);
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      const int row0 = tm * kPairBM + cta_rank * BM + q * 32;
+      const int rows = p.T - row0;
+      const uint32_t taddr = tmem_base + acc * kAccCols + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; c < kHCols; c += 64) {
+        const int col0 = tn * kHCols + c, cols = p.F - col0;
+        // one 64-column group goes through the patch up to three times: gate, up (for the backward pass), h
+#pragma unroll 1
+        for (int what = p.gu ? 0 : 2; what < 3; ++what) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t r[32];
+            float v[32];
+            if (what != 1) {
+              tmem_ld_32x32(taddr + c + half * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+            }
+            if (what != 0) {
+              tmem_ld_32x32(taddr + kHCols + c + half * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                v[i] = what == 1 ? __uint_as_float(r[i]) : activate(p.act, v[i]) * __uint_as_float(r[i]);
+            }
+            patch_put(patch, lane, half, v);
+          }
+          __nv_bfloat16* base = what == 2 ? p.h + (int64_t)row0 * p.ldh + col0
+                                          : p.gu + (int64_t)row0 * p.ldgu + (what ? p.F : 0) + col0;
+          patch_store(patch, lane, base, what == 2 ? p.ldh : p.ldgu, rows, cols);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[acc]), 0));
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+  }
+
+  body_sync();
+  if (*abort_flag) {
+    // a wait ran out: give copies that may still be in flight time to land before this shared memory is released
+    for (int i = 0; i < 64; ++i) __nanosleep(20000);
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();  // the peer no longer reads this CTA's shared memory or signals its barriers
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace gated
+}  // namespace mb

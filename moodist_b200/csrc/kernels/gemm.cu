@@ -89,7 +89,8 @@ int fill_params_and_maps(Params& p, CUtensorMap& ta, CUtensorMap& tb, const void
                          int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int a_mn, int b_mn, int out_fp32,
                          int epilogue, uint32_t* status, uint64_t wait_ns) {
   if (M <= 0 || N <= 0 || K <= 0) return MB_ERR_ARG;
-  if ((N % 8) || (K % 8) || (M % 8 && a_mn)) return MB_ERR_ALIGN;
+  // K is a row count when both operands are MN-major (a weight gradient over any number of tokens): TMA fills the rest
+  if ((N % 8) || (K % 8 && !(a_mn && b_mn)) || (M % 8 && a_mn)) return MB_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(C) & 15) || ((ldc * (out_fp32 ? 4 : 2)) & 15)) return MB_ERR_ALIGN;
   int rc;
   // K-major operand: matrix [MN, K], box 64(k) x tile rows.  MN-major: matrix [K, MN], box 64(mn) x 64(k).

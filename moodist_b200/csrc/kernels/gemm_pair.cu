@@ -74,7 +74,8 @@ int gemm_pair_launch(const void* A, const void* B, void* C, int M, int N, int K,
                      int a_mn, int b_mn, int out_fp32, int epilogue, uint32_t* status, uint64_t wait_ns,
                      cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0) return MB_ERR_ARG;
-  if ((N % 8) || (K % 8) || (M % 8 && a_mn)) return MB_ERR_ALIGN;
+  // K is a row count when both operands are MN-major (a weight gradient over any number of tokens): TMA fills the rest
+  if ((N % 8) || (K % 8 && !(a_mn && b_mn)) || (M % 8 && a_mn)) return MB_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(C) & 15) || ((ldc * (out_fp32 ? 4 : 2)) & 15)) return MB_ERR_ALIGN;
   CUtensorMap ta, tb;
   int rc = a_mn ? make_tmap_bf16(&ta, A, K, M, lda, 64) : make_tmap_bf16(&ta, A, M, K, lda, BM);

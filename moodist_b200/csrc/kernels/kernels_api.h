@@ -203,6 +203,74 @@ int mb_rmsnorm_bwd_bf16(const void* x, const void* w, const void* dy, const floa
 int mb_adamw_bf16(void* p, const void* g, int grad_dtype, void* m, void* v, int64_t n, float lr, float b1, float b2,
                   float eps, float wd, int step, float grad_scale, void* stream);
 
+// --- decoder operators: MB_BF16, MB_F16 or MB_F32 tensors whose last dimension is contiguous; strides in elements -------
+// Layer normalisation over the last dimension (norm_ops.cu). w and b (each may be null) are of w_dtype: the rows' type or
+// MB_F32. mean and rstd (both null when no backward pass follows) receive the row statistics.
+int mb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D,
+                     int64_t x_stride, int64_t y_stride, int dtype, int w_dtype, float eps, void* stream);
+// dx, dw and db may each be null; `partial` is fp32 scratch of mb_layernorm_bwd_parts(rows, D) x 2 x D elements when dw or
+// db is wanted. rows = 0 writes nothing, dw and db included.
+int mb_layernorm_bwd_parts(int64_t rows, int64_t D);
+int mb_layernorm_bwd(const void* x, const void* w, const void* dy, const float* mean, const float* rstd, void* dx, void* dw,
+                     void* db, float* partial, int64_t rows, int64_t D, int64_t x_stride, int64_t dy_stride,
+                     int64_t dx_stride, int dtype, int w_dtype, void* stream);
+// Rotary positions on q[batch, seq, q_heads, dim] and k[batch, seq, k_heads, dim] (rotary.cu): dimensions [0, rot) turn by
+// the angle of the token's position, in pairs (j, j + rot/2) or, interleaved, (2j, 2j + 1). cos_tab / sin_tab are contiguous
+// fp32 [length, rot/2]. positions (null: 0 .. seq-1): a negative one leaves its token as it is, one from `length` up gives NaN.
+typedef struct {
+  const void* in;
+  void* out;  // == in when in_place
+  int64_t in_batch, in_seq, in_head, out_batch, out_seq, out_head;
+} mb_rotary_heads_t;
+typedef struct {
+  mb_rotary_heads_t q, k;
+  int64_t batch, seq;
+  int q_heads, k_heads;  // either may be 0
+  int dim, rot, dtype;
+  int interleaved, inverse, in_place;
+  const float* cos_tab;
+  const float* sin_tab;
+  int64_t length;
+  const void* positions;
+  int64_t pos_batch, pos_seq;
+  int pos_i64;  // 0: int32
+} mb_rotary_t;
+int mb_rotary(const mb_rotary_t* p, void* stream);
+
+// Distillation from a teacher's top entries (distill.cu). logits[rows, V]; ids and top are contiguous [rows, K], an id outside
+// [0, V) and an entry at -inf are padding; targets (may be null) is contiguous [rows], a row whose target is ignore_index or outside [0, V), and a
+// row without any valid entry, is left out. Row loss = (1 - hard) tau^2 sum_k p_k (log p_k - log q_k) + hard (lse - z_target)
+// with p = softmax(top / tau) over the valid entries and q = softmax(z / tau).
+typedef struct {
+  const void* logits;
+  int64_t rows, stride;
+  int V, K;
+  int dtype, top_dtype, ids_i64;
+  const void* ids;
+  const void* top;
+  const int64_t* targets;
+  int64_t ignore_index;
+  float tau, hard, scale;
+  int mean;        // 1: over the rows that take part, 0: sum
+  float* p;        // scratch [rows, K]: the teacher's probabilities
+  float* entropy;  // scratch [rows]: sum_k p_k log p_k
+  int* live;       // scratch [rows]
+  float* factor;   // [1]: scale, or scale / number of rows that take part
+  float* stats;    // [rows, 3]: max, 1 / sum exp((z - max) / tau), 1 / sum exp(z - max)
+  float* row_loss; // scratch [rows]
+  float* loss;     // [1]
+} mb_distill_t;
+int mb_distill_fwd(const mb_distill_t* d, void* stream);
+// grad[rows, V] = d loss / d logits * gout[0], from the p, live, factor and stats that the forward call left
+int mb_distill_bwd(const mb_distill_t* d, const float* gout, void* grad, int64_t grad_stride, void* stream);
+// Gated projection (gated_gemm.cu): h[T, F] = act(x Wg^T) * (x Wu^T) for bf16 x[T, K] and w[2F, K] (gate rows first); gu
+// (may be null) receives the two projections [T, 2F]. act: 0 SiLU, 1 GELU, 2 GELU with tanh. F, K and the pitches are
+// multiples of 8, all addresses 16-byte aligned. The backward call turns dh and gu into dgu[T, 2F], the gradient of x w^T.
+int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, int64_t T, int F, int K, int64_t ldx, int64_t ldw,
+                      int64_t ldh, int64_t ldgu, int act, uint32_t* status, uint64_t wait_ns, void* stream);
+int mb_gated_bwd_bf16(const void* gu, const void* dh, void* dgu, int64_t T, int F, int64_t ldgu, int64_t lddh, int64_t lddgu,
+                      int act, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,8 @@ transposed in memory.  There is no fallback: on a CUDA device the extension must
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .._core import _C
@@ -78,6 +80,28 @@ class _Linear(torch.autograd.Function):
 def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """``x @ w.T`` for bf16 CUDA tensors; differentiable in both arguments."""
     return _Linear.apply(x, w)
+
+
+def gated_linear(x: torch.Tensor, w: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """``act(x @ Wg.T) * (x @ Wu.T)`` for ``x[..., K]`` and ``w[2F, K]`` (gate rows ``[0, F)``, up rows ``[F, 2F)``, the layout
+    of ``swiglu(linear(x, w))``): both projections, the activation and the product in one tcgen05 kernel.
+
+    bf16, ``F`` and ``K`` multiples of 8, any number of rows; ``activation`` is ``"silu"``, ``"gelu"`` or ``"gelu_tanh"``.
+    The result is rounded once from fp32.  Differentiable (once) in both arguments: the forward pass then keeps the two
+    projections in bf16 and the backward pass is one elementwise kernel and two matrix products.
+    """
+    if x.is_cuda:
+        return _C.gated_linear(x, w, activation)
+    _C.gated_check(x, w, activation)
+    g, u = (x.float() @ w.float().t()).chunk(2, dim=-1)
+    # erfc and the logistic form keep the left tail's relative accuracy, which 1 + erf and 1 + tanh cancel away
+    if activation == "silu":
+        a = g * torch.sigmoid(g)
+    elif activation == "gelu":
+        a = 0.5 * g * torch.special.erfc(-g * math.sqrt(0.5))
+    else:
+        a = g * torch.sigmoid(math.sqrt(8 / math.pi) * (g + 0.044715 * g**3))
+    return (a * u).to(x.dtype)
 
 
 class Linear(torch.nn.Module):

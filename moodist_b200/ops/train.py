@@ -6,13 +6,20 @@
                   gradient, so no fp32 copy of the ``[tokens, vocab]`` matrix is ever made
 ``adamw_``        AdamW over a flat bf16 parameter shard with bf16 moments (gradient fp32 or bf16)
 ``rms_norm``      RMSNorm over the last dimension; the backward produces dx and dw in one pass over dy and x
+``layer_norm``    layer normalisation over the last dimension with optional weight and bias, any width
+``rotary``        rotary positions on q and k in one launch: either pair layout, part of the head, a position per token;
+                  ``rotary_`` in place for serving, ``rotary_tables`` with the scalings for long contexts
+``distill_loss``  distillation from a teacher's top logits, alone or with the hard targets' cross-entropy
 
-On CUDA tensors these always run the kernels of ``csrc/kernels/train_ops.cu``.  CPU tensors take plain
-PyTorch arithmetic so the sharded engine's host-side logic can be exercised on ``gloo`` ranks.
+On CUDA tensors these always run the kernels of ``csrc/kernels/`` (``train_ops.cu``, ``norm_ops.cu``, ``rotary.cu``,
+``distill.cu``).  CPU tensors take plain PyTorch arithmetic so the sharded engine's host-side logic can be exercised on
+``gloo`` ranks.
 The reference library is a communication backend and has no counterpart of these ops.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn.functional as F
@@ -24,7 +31,7 @@ _launches = 0
 
 def train_op_launches() -> int:
     """Number of kernels launched by this module so far in this process."""
-    return _launches
+    return _launches + _C.decoder_op_launches()
 
 
 def _count(n: int = 1) -> None:
@@ -225,3 +232,143 @@ def adamw_master_(p, master, g, m, v, lr: float, betas=(0.9, 0.95), eps: float =
     denom = v.sqrt().div_(bc2**0.5).add_(eps)
     master.mul_(1 - lr * weight_decay).addcdiv_(m, denom, value=-lr / bc1)
     p.copy_(master)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension; differentiable (once) in all three.
+
+    ``x`` is bf16, fp16 or fp32 with any leading dimensions and any width; ``weight`` and ``bias`` are ``[width]``, both of
+    ``x``'s type or both fp32, and may be left out.  Statistics and the sums of the weight's and bias's gradients are fp32
+    with a fixed order of summation.
+    """
+    if x.is_cuda:
+        return _C.layer_norm(x, weight, bias, eps)
+    _C.layer_norm_check(x, weight, bias, eps)
+    w = None if weight is None else weight.float()
+    b = None if bias is None else bias.float()
+    return F.layer_norm(x.float(), (x.shape[-1],), w, b, eps).to(x.dtype)
+
+
+def rotary_tables(rotary_dim: int, length: int, theta: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                  original_length: int | None = None, low: float = 1.0, high: float = 4.0, device=None):
+    """fp32 ``(cos, sin)`` tables ``[length, rotary_dim / 2]`` for :func:`rotary`, the angles computed in 64 bits.
+
+    ``scaling`` stretches a model to contexts ``factor`` times longer than it was trained on: ``"linear"`` divides every
+    angle by ``factor``; ``"ntk"`` raises the base to ``theta * factor ** (R / (R - 2))``, which divides the lowest
+    frequency by ``factor`` and leaves the highest; ``"by_parts"`` leaves a frequency that turns ``high`` times or more
+    within ``original_length`` positions, divides one that turns ``low`` times or less, and blends in between.
+    """
+    if rotary_dim < 2 or rotary_dim % 2 or length < 1:
+        raise ValueError("moodist rotary_tables: an even rotary_dim and a length of at least 1 are required")
+    if scaling not in (None, "linear", "ntk", "by_parts"):
+        raise ValueError(f"moodist rotary_tables: unknown scaling {scaling!r}")
+    if not theta > 0 or not factor > 0:
+        raise ValueError("moodist rotary_tables: theta and factor must be positive")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("moodist rotary_tables: ntk scaling needs a rotary_dim of at least 4")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    inv = theta ** (-torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64) / rotary_dim)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "by_parts":
+        if original_length is None or original_length < 1 or not 0 <= low < high:
+            raise ValueError("moodist rotary_tables: by_parts needs original_length and 0 <= low < high")
+        turns = original_length * inv / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        inv = inv * (keep + (1 - keep) / factor)
+    angle = torch.outer(torch.arange(length, device=device, dtype=torch.float64), inv)
+    return angle.cos().float(), angle.sin().float()
+
+
+def _turn_reference(x, cos, sin, positions, interleaved):
+    length, half = cos.shape
+    seq = x.shape[-3]
+    pos = torch.arange(seq, device=x.device) if positions is None else positions.long()
+    at = pos.clamp(0, length - 1)
+    still, beyond = (pos < 0)[..., None, None], (pos >= length)[..., None, None]
+    c, s = cos[at][..., None, :], sin[at][..., None, :]
+    head = x[..., : 2 * half].float()
+    a, b = (head[..., 0::2], head[..., 1::2]) if interleaved else (head[..., :half], head[..., half:])
+    ta, tb = a * c - b * s, b * c + a * s
+    turned = torch.stack([ta, tb], -1).flatten(-2) if interleaved else torch.cat([ta, tb], -1)
+    turned = torch.where(still, head, torch.where(beyond, float("nan"), turned))
+    return torch.cat([turned.to(x.dtype), x[..., 2 * half :]], -1)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None,
+           interleaved: bool = False):
+    """``(q', k')``: rotary positions on ``q[B, S, H, D]`` and ``k[B, S, KV, D]`` (or without ``B``); ``k`` may be None.
+
+    ``cos`` / ``sin`` are fp32 ``[positions, R / 2]`` (:func:`rotary_tables`): the first ``R <= D`` dimensions of a head turn,
+    in pairs ``(j, j + R/2)`` or, ``interleaved``, ``(2j, 2j + 1)``, the others pass through.  ``positions`` (int64 or int32,
+    ``[B, S]`` or ``[S]``; default ``0 .. S-1``) says where each token stands; a negative one marks padding, which passes
+    through unchanged, and one that the tables do not have gives NaN.  bf16, fp16 or fp32, any strides (views of a fused
+    projection's output go in as they are); the results are new contiguous tensors.  Differentiable (once) in q and k.
+    """
+    if q.is_cuda:
+        return _C.rotary(q, k, cos, sin, positions, interleaved)
+    _C.rotary_check(q, k, cos, sin, positions)
+    return (_turn_reference(q, cos, sin, positions, interleaved),
+            None if k is None else _turn_reference(k, cos, sin, positions, interleaved))
+
+
+def rotary_(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None,
+            interleaved: bool = False) -> None:
+    """:func:`rotary` written over ``q`` and ``k``, for serving (no gradient passes through it).  Dimensions from ``R`` up and
+    tokens at negative positions are not touched."""
+    if q.is_cuda:
+        _C.rotary_(q, k, cos, sin, positions, interleaved)
+        return
+    _C.rotary_check(q, k, cos, sin, positions)
+    _C.rotary_in_place_check(q, k)
+    for x in (q, k):
+        if x is not None:
+            x.copy_(_turn_reference(x, cos, sin, positions, interleaved))
+
+
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, targets: torch.Tensor | None = None, *,
+                 temperature: float = 1.0, hard_weight: float = 0.0, ignore_index: int = -100, reduction: str = "mean",
+                 scale: float = 1.0) -> torch.Tensor:
+    """Distillation loss of ``logits[..., V]`` against a teacher's top entries ``teacher_ids`` / ``teacher_logits[..., K]``.
+
+    Per row ``(1 - hard_weight) * temperature^2 * KL(p || q) + hard_weight * cross_entropy(logits, targets)`` where ``p`` is
+    the softmax of the teacher's entries over ``temperature`` (renormalised over the entries given) and ``q`` the softmax of
+    ``logits / temperature`` over the vocabulary.  An entry whose id is outside ``[0, V)`` or whose logit is ``-inf`` is
+    padding; a word named twice counts with both entries.  A row without any entry, or whose target is ``ignore_index`` (or
+    outside ``[0, V)``), gives neither loss nor gradient.  The fp32 result is the sum over the other rows, or their mean
+    (0 when there is none), times ``scale``.
+
+    Logits are bf16, fp16 or fp32, ids int64 or int32, teacher logits bf16, fp16 or fp32, targets int64.  Differentiable
+    (once) in ``logits``, which stay as they are: where :func:`cross_entropy` is wanted as well, take it in here through
+    ``targets``, since its own backward pass overwrites the logits that this one reads.
+    """
+    if reduction not in ("mean", "sum"):
+        raise ValueError(f"moodist distill_loss: reduction must be 'mean' or 'sum', not {reduction!r}")
+    if logits.is_cuda:
+        return _C.distill_loss(logits, teacher_ids, teacher_logits, targets, temperature, hard_weight, ignore_index,
+                               reduction == "mean", scale)
+    _C.distill_check(logits, teacher_ids, teacher_logits, targets, temperature, hard_weight)
+    V, K = logits.shape[-1], teacher_ids.shape[-1]
+    ids, top = teacher_ids.reshape(-1, K).long(), teacher_logits.reshape(-1, K).float()
+    valid = (ids >= 0) & (ids < V) & (top != float("-inf"))
+    live = valid.any(-1)
+    if targets is not None:
+        t = targets.reshape(-1)
+        live = live & (t != ignore_index) & (t >= 0) & (t < V)
+    valid = valid & live[:, None]
+    z = torch.where(live[:, None], logits.reshape(-1, V).float(), 0.0)
+    at = torch.where(valid, ids, 0)
+    top = torch.where(valid, top / temperature, float("-inf"))
+    peak = torch.where(live, top.amax(-1), 0.0)[:, None]
+    logp = top - peak - torch.where(live, (top - peak).exp().sum(-1), 1.0).log()[:, None]
+    p = logp.exp()
+    rows = z.new_zeros(z.shape[0])
+    if hard_weight < 1:
+        logq = torch.log_softmax(z / temperature, -1).gather(1, at)
+        term = torch.where(p == 0, 0.0, p * (torch.where(p == 0, 0.0, logp) - torch.where(p == 0, 0.0, logq)))
+        rows = rows + (1 - hard_weight) * temperature**2 * term.sum(-1)
+    if hard_weight > 0:
+        rows = rows + hard_weight * F.cross_entropy(z, torch.where(live, t, 0), reduction="none")
+    factor = scale / live.sum().clamp(min=1) if reduction == "mean" else scale
+    return torch.where(live, rows, 0.0).sum() * factor
