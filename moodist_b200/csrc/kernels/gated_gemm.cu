@@ -13,15 +13,18 @@ namespace gated {
 
 constexpr int kMaxDevices = 64;
 
+template <int kAct, bool kSave>
 __global__ void __launch_bounds__(kNumThreads, 1)
     gated_pair_kernel(const __grid_constant__ GatedParams p, const __grid_constant__ CUtensorMap tmap_x,
                       const __grid_constant__ CUtensorMap tmap_w) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  gated_pair_body(p, &tmap_x, &tmap_w, smem_raw);
+  gated_pair_body<kAct, kSave>(p, &tmap_x, &tmap_w, smem_raw);
 }
 
+template <int kAct, bool kSave>
 static int launch_pair(GatedParams& p, const CUtensorMap& tx, const CUtensorMap& tw, int device, cudaStream_t stream) {
-  static int max_clusters[kMaxDevices];  // 0: not asked yet
+  auto kern = gated_pair_kernel<kAct, kSave>;
+  static int max_clusters[kMaxDevices];  // per instantiation; 0: not asked yet
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -29,17 +32,17 @@ static int launch_pair(GatedParams& p, const CUtensorMap& tx, const CUtensorMap&
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.blockDim = dim3(kNumThreads, 1, 1);
-  cfg.dynamicSmemBytes = kPairSmemBytes;
+  cfg.dynamicSmemBytes = kGatedPairSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (max_clusters[device] == 0) {
     int sms = 0, n = 0;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-        cudaFuncSetAttribute(gated_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes) != cudaSuccess)
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGatedPairSmem) != cudaSuccess)
       return MB_ERR_LAUNCH;
     cfg.gridDim = dim3(sms & ~1, 1, 1);
-    if (cudaOccupancyMaxActiveClusters(&n, gated_pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       n = sms / 2;
     }
@@ -48,7 +51,7 @@ static int launch_pair(GatedParams& p, const CUtensorMap& tx, const CUtensorMap&
   const int tiles = p.tiles_m * p.tiles_n;
   p.num_ctas = 2 * (tiles < max_clusters[device] ? tiles : max_clusters[device]);
   cfg.gridDim = dim3(p.num_ctas, 1, 1);
-  return cudaLaunchKernelEx(&cfg, gated_pair_kernel, p, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kern, p, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
 // dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F], bound by their bytes.
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__(256)
     load_vec<__nv_bfloat16, 8>(dh + t * lddh + j, d);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float2 a = activate_slope(kAct, g[k]);
+      const float2 a = activate_slope<kAct>(g[k]);
       g[k] = d[k] * u[k] * a.y;
       u[k] = d[k] * a.x;
     }
@@ -104,13 +107,20 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   p.ldh = ldh;
   p.gu = (__nv_bfloat16*)gu;
   p.ldgu = ldgu;
-  p.act = act;
   p.tiles_m = (int)((T + kPairBM - 1) / kPairBM);
   p.tiles_n = (F + kHCols - 1) / kHCols;
   p.group_m = 4;
   p.status = status;
   p.wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
-  return launch_pair(p, tx, tw, device, MB_STREAM(stream));
+  cudaStream_t s = MB_STREAM(stream);
+  switch (act * 2 + (gu ? 1 : 0)) {
+    case 0: return launch_pair<kSilu, false>(p, tx, tw, device, s);
+    case 1: return launch_pair<kSilu, true>(p, tx, tw, device, s);
+    case 2: return launch_pair<kGelu, false>(p, tx, tw, device, s);
+    case 3: return launch_pair<kGelu, true>(p, tx, tw, device, s);
+    case 4: return launch_pair<kGeluTanh, false>(p, tx, tw, device, s);
+    default: return launch_pair<kGeluTanh, true>(p, tx, tw, device, s);
+  }
 }
 
 extern "C" int mb_gated_bwd_bf16(const void* gu, const void* dh, void* dgu, int64_t T, int F, int64_t ldgu, int64_t lddh,

@@ -36,7 +36,6 @@ struct GatedParams {
   int64_t ldh;
   __nv_bfloat16* gu;  // [T, 2F] or null
   int64_t ldgu;
-  int act;
   int tiles_m, tiles_n, group_m;
   int num_ctas;
   uint32_t* status;
@@ -44,19 +43,20 @@ struct GatedParams {
 };
 
 // act(g); the logistic form of the tanh approximation and erfc keep the relative accuracy of the left tail
-__device__ __forceinline__ float activate(int act, float g) {
-  if (act == kSilu) return g / (1.f + __expf(-g));
-  if (act == kGelu) return g * 0.5f * erfcf(-g * 0.70710678f);
-  const float y2 = 1.5957691216f * (g + 0.044715f * g * g * g);
-  return g / (1.f + __expf(-y2));
+template <int kAct>
+__device__ __forceinline__ float activate(float g) {
+  if (kAct == kGelu) return g * 0.5f * erfcf(-g * 0.70710678f);
+  const float y = kAct == kSilu ? g : 1.5957691216f * (g + 0.044715f * g * g * g);
+  return __fdividef(g, 1.f + __expf(-y));
 }
 // act(g) and its derivative
-__device__ __forceinline__ float2 activate_slope(int act, float g) {
-  if (act == kSilu) {
+template <int kAct>
+__device__ __forceinline__ float2 activate_slope(float g) {
+  if (kAct == kSilu) {
     const float s = 1.f / (1.f + __expf(-g));
     return make_float2(g * s, s * (1.f + g * (1.f - s)));
   }
-  if (act == kGelu) {
+  if (kAct == kGelu) {
     const float c = 0.5f * erfcf(-g * 0.70710678f);
     return make_float2(g * c, c + g * __expf(-0.5f * g * g) * 0.39894228f);
   }
@@ -80,27 +80,74 @@ __device__ __forceinline__ void gated_tile(const GatedParams& p, int t, int& tm,
   tn = r / gsz;
 }
 
-// 32 values of a lane's row -> its line of the warp's patch, half `h` of 64 columns
-__device__ __forceinline__ void patch_put(uint8_t* patch, int lane, int h, const float* v) {
-  uint4* dst = reinterpret_cast<uint4*>(patch + lane * kEpiRowBytes + h * 64);
+// The epilogue's patch of shared memory per warp: 32 rows of three 64-byte pieces (32 columns of h, gate and up), padded so
+// that 16-byte accesses of eight rows meet no bank twice.
+constexpr int kPatchRow = 208;
+constexpr int kPatchBytes = 32 * kPatchRow;
+constexpr int kGatedPairSmem = kPairStages * kPairStageBytes + 1024 + 256 + 4 * kPatchBytes;
+
+// 16 values of a lane's row -> 32 bytes of its line
+__device__ __forceinline__ void patch_put(uint8_t* to, const float* v) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
-    dst[g] = make_uint4(pack_bf16x2(v[g * 8], v[g * 8 + 1]), pack_bf16x2(v[g * 8 + 2], v[g * 8 + 3]),
-                        pack_bf16x2(v[g * 8 + 4], v[g * 8 + 5]), pack_bf16x2(v[g * 8 + 6], v[g * 8 + 7]));
+  for (int g = 0; g < 2; ++g)
+    reinterpret_cast<uint4*>(to)[g] =
+        make_uint4(pack_bf16x2(v[g * 8], v[g * 8 + 1]), pack_bf16x2(v[g * 8 + 2], v[g * 8 + 3]),
+                   pack_bf16x2(v[g * 8 + 4], v[g * 8 + 5]), pack_bf16x2(v[g * 8 + 6], v[g * 8 + 7]));
 }
-// the patch's 32 rows x 64 columns -> global memory as 128-byte lines
-__device__ __forceinline__ void patch_store(const uint8_t* patch, int lane, __nv_bfloat16* base, int64_t ld, int rows, int cols) {
-  __syncwarp();
-  const int col = (lane & 7) * 8;
+// one piece of the patch, 32 rows x 32 columns -> global memory, whole 64-byte runs
+__device__ __forceinline__ void patch_store(const uint8_t* piece, int lane, __nv_bfloat16* base, int64_t ld, int rows, int cols) {
+  const int col = (lane & 3) * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int rr = i * 4 + (lane >> 3);
-    const uint4 v = *reinterpret_cast<const uint4*>(patch + rr * kEpiRowBytes + (lane & 7) * 16);
+  for (int i = 0; i < 4; ++i) {
+    const int rr = i * 8 + (lane >> 2);
+    const uint4 v = *reinterpret_cast<const uint4*>(piece + rr * kPatchRow + (lane & 3) * 16);
     if (rr < rows && col < cols) *reinterpret_cast<uint4*>(base + (int64_t)rr * ld + col) = v;
   }
-  __syncwarp();
 }
 
+// The warp's 32 rows x `width` columns of h from the accumulator at `taddr` (gate columns, up columns `up` further on):
+// sixteen columns at a time in a rolled loop, because code that is run once per tile from a cold instruction cache costs
+// more than the arithmetic (the fully unrolled form took 60 us for one tile).
+template <int kAct, bool kSave>
+__device__ __forceinline__ void gated_epilogue(const GatedParams& p, uint32_t taddr, int up, int width, uint8_t* patch, int lane,
+                                               int row0, int col0) {
+  const int rows = p.T - row0;
+#pragma unroll 1
+  for (int c = 0; c < width; c += 32) {
+    const int cols = min(p.F - (col0 + c), width - c);
+    uint8_t* line = patch + lane * kPatchRow;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      uint32_t rg[16], ru[16];
+      tmem_ld_32x16(taddr + c + half * 16, rg);
+      tmem_ld_32x16(taddr + up + c + half * 16, ru);
+      tmem_ld_wait();
+      float g[16], u[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        g[i] = __uint_as_float(rg[i]);
+        u[i] = __uint_as_float(ru[i]);
+      }
+      if (kSave) {
+        patch_put(line + 64 + half * 32, g);
+        patch_put(line + 128 + half * 32, u);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) g[i] = activate<kAct>(g[i]) * u[i];
+      patch_put(line + half * 32, g);
+    }
+    __syncwarp();
+    patch_store(patch, lane, p.h + (int64_t)row0 * p.ldh + col0 + c, p.ldh, rows, cols);
+    if (kSave) {
+      __nv_bfloat16* to = p.gu + (int64_t)row0 * p.ldgu + col0 + c;
+      patch_store(patch + 64, lane, to, p.ldgu, rows, cols);
+      patch_store(patch + 128, lane, to + p.F, p.ldgu, rows, cols);
+    }
+    __syncwarp();
+  }
+}
+
+template <int kAct, bool kSave>
 __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUtensorMap* tmap_x, const CUtensorMap* tmap_w,
                                                 uint8_t* smem_raw) {
   uint32_t raw = smem_u32(smem_raw);
@@ -204,7 +251,7 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
     }
   } else {
     const int q = warp & 3;  // TMEM lane quarter this warp may read
-    uint8_t* patch = epi_patch + (warp - 2) * kEpiPatchBytes;
+    uint8_t* patch = epi_patch + (warp - 2) * kPatchBytes;
     uint32_t local_tile = 0;
     bool ok = true;
     for (int t = pair; t < num_tiles; t += stride, ++local_tile) {
@@ -217,39 +264,8 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
         break;
       }
       tc_fence_after_sync();
-      const int row0 = tm * kPairBM + cta_rank * BM + q * 32;
-      const int rows = p.T - row0;
-      const uint32_t taddr = tmem_base + acc * kAccCols + ((uint32_t)(q * 32) << 16);
-#pragma unroll 1
-      for (int c = 0; c < kHCols; c += 64) {
-        const int col0 = tn * kHCols + c, cols = p.F - col0;
-        // one 64-column group goes through the patch up to three times: gate, up (for the backward pass), h
-#pragma unroll 1
-        for (int what = p.gu ? 0 : 2; what < 3; ++what) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t r[32];
-            float v[32];
-            if (what != 1) {
-              tmem_ld_32x32(taddr + c + half * 32, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-            }
-            if (what != 0) {
-              tmem_ld_32x32(taddr + kHCols + c + half * 32, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                v[i] = what == 1 ? __uint_as_float(r[i]) : activate(p.act, v[i]) * __uint_as_float(r[i]);
-            }
-            patch_put(patch, lane, half, v);
-          }
-          __nv_bfloat16* base = what == 2 ? p.h + (int64_t)row0 * p.ldh + col0
-                                          : p.gu + (int64_t)row0 * p.ldgu + (what ? p.F : 0) + col0;
-          patch_store(patch, lane, base, what == 2 ? p.ldh : p.ldgu, rows, cols);
-        }
-      }
+      gated_epilogue<kAct, kSave>(p, tmem_base + acc * kAccCols + ((uint32_t)(q * 32) << 16), kHCols, kHCols, patch, lane,
+                                  tm * kPairBM + cta_rank * BM + q * 32, tn * kHCols);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[acc]), 0));
