@@ -54,6 +54,41 @@ static int launch_pair(GatedParams& p, const CUtensorMap& tx, const CUtensorMap&
   return cudaLaunchKernelEx(&cfg, kern, p, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
+template <int kAct, bool kSave>
+__global__ void __launch_bounds__(kNumThreads, 1)
+    gated_rows_kernel(const __grid_constant__ GatedParams p, int width, int x_rows, const __grid_constant__ CUtensorMap tmap_x,
+                      const __grid_constant__ CUtensorMap tmap_w) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  gated_rows_body<kAct, kSave>(p, width, x_rows, &tmap_x, &tmap_w, smem_raw);
+}
+
+template <int kAct, bool kSave>
+static int launch_rows(const GatedParams& p, int width, int x_rows, const CUtensorMap& tx, const CUtensorMap& tw, int device,
+                       cudaStream_t stream) {
+  auto kern = gated_rows_kernel<kAct, kSave>;
+  static bool configured[kMaxDevices];  // per instantiation
+  if (!configured[device]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) != cudaSuccess) return MB_ERR_LAUNCH;
+    configured[device] = true;
+  }
+  kern<<<(p.F + width - 1) / width, kNumThreads, kRowsSmem, stream>>>(p, width, x_rows, tx, tw);
+  return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+}
+
+// Columns of h per CTA in the few-rows kernel: the narrowest multiple of 8 with which as few waves as 128 columns would
+// need cover F.
+static int rows_width(int F, int device) {
+  static int sms[kMaxDevices];
+  if (sms[device] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
+    sms[device] = n;
+  }
+  const int waves = (F + 128 * sms[device] - 1) / (128 * sms[device]);
+  const int ctas = waves * sms[device];
+  return ((F + ctas - 1) / ctas + 7) / 8 * 8;
+}
+
 // dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F], bound by their bytes.
 // The results are rounded to bf16 because the two matrix products that follow take bf16 operands.
 template <int kAct>
@@ -94,10 +129,14 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   if (!is_aligned(x, 16) || !is_aligned(w, 16) || !is_aligned(h, 16) || !is_aligned(gu, 16)) return MB_ERR_ALIGN;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return MB_ERR_DRIVER;
+  // Few rows: the weight's bytes bound the time and a 256-row tile would leave SMs idle (one token, F = 14336, K = 4096:
+  // 65 us in pair tiles).
+  const bool few = T <= BM;
+  const int width = few ? rows_width(F, device) : kHCols, x_rows = few ? (int)(T + 7) / 8 * 8 : BM;
   CUtensorMap tx, tw;
-  int rc = gemm::make_tmap_bf16(&tx, x, T, K, ldx, BM);
+  int rc = gemm::make_tmap_bf16(&tx, x, T, K, ldx, x_rows);
   if (rc) return rc;
-  rc = gemm::make_tmap_bf16(&tw, w, 2 * (uint64_t)F, K, ldw, kHCols);
+  rc = gemm::make_tmap_bf16(&tw, w, 2 * (uint64_t)F, K, ldw, width);
   if (rc) return rc;
   GatedParams p{};
   p.T = (int)T;
@@ -114,12 +153,12 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   p.wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
   cudaStream_t s = MB_STREAM(stream);
   switch (act * 2 + (gu ? 1 : 0)) {
-    case 0: return launch_pair<kSilu, false>(p, tx, tw, device, s);
-    case 1: return launch_pair<kSilu, true>(p, tx, tw, device, s);
-    case 2: return launch_pair<kGelu, false>(p, tx, tw, device, s);
-    case 3: return launch_pair<kGelu, true>(p, tx, tw, device, s);
-    case 4: return launch_pair<kGeluTanh, false>(p, tx, tw, device, s);
-    default: return launch_pair<kGeluTanh, true>(p, tx, tw, device, s);
+    case 0: return few ? launch_rows<kSilu, false>(p, width, x_rows, tx, tw, device, s) : launch_pair<kSilu, false>(p, tx, tw, device, s);
+    case 1: return few ? launch_rows<kSilu, true>(p, width, x_rows, tx, tw, device, s) : launch_pair<kSilu, true>(p, tx, tw, device, s);
+    case 2: return few ? launch_rows<kGelu, false>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGelu, false>(p, tx, tw, device, s);
+    case 3: return few ? launch_rows<kGelu, true>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGelu, true>(p, tx, tw, device, s);
+    case 4: return few ? launch_rows<kGeluTanh, false>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGeluTanh, false>(p, tx, tw, device, s);
+    default: return few ? launch_rows<kGeluTanh, true>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGeluTanh, true>(p, tx, tw, device, s);
   }
 }
 

@@ -286,5 +286,125 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
   }
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------------------
+// Up to 128 rows the weight's bytes are the bound (4 F K of them: 36 us at F = 14336, K = 4096 and the measured copy rate),
+// and a 256-row tile leaves most SMs without one. Here a single CTA computes all rows of `width` columns of h, with the width
+// chosen so that one wave of CTAs covers F; 128 x 2 width accumulators, gate columns first. Only the rows of x that exist
+// are loaded (rounded up to 8): the tensor core reads what lies in the other rows of the 128-row operand, whose results
+// nothing looks at.
+enum RowsStatus : uint32_t {
+  kTimeoutRowsProducer = 0x131,
+  kTimeoutRowsMma = 0x132,
+  kTimeoutRowsEpilogue = 0x133,
+  kTimeoutRowsDrain = 0x134,
+};
+constexpr int kRowsMaxStages = 8;
+constexpr int kRowsSmem = 227 * 1024;
+constexpr int kRowsTmemCols = 256;
+
+__host__ __device__ inline int rows_stage_bytes(int width) { return kATileBytes + 2 * width * 128; }
+__host__ __device__ inline int rows_stages(int width) {
+  const int n = (kRowsSmem - 1024 - 256) / rows_stage_bytes(width);
+  return n < kRowsMaxStages ? n : kRowsMaxStages;
+}
+
+template <int kAct, bool kSave>
+__device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width, int x_rows, const CUtensorMap* tmap_x,
+                                                const CUtensorMap* tmap_w, uint8_t* smem_raw) {
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* tiles = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const int stages = rows_stages(width), stage_bytes = rows_stage_bytes(width);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);  // [stages]
+  uint64_t* empty = full + kRowsMaxStages;                                     // [stages]
+  uint64_t* acc_full = empty + kRowsMaxStages;
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kblocks = (p.K + BK - 1) / BK;
+  const int col0 = blockIdx.x * width;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(tmap_x);
+    tma_prefetch_desc(tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_base_slot, kRowsTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  body_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_base_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0;
+      for (; it < kblocks; ++it) {
+        const int s = it % stages;
+        if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, p.wait_ns)) {
+          gated_report(p, kTimeoutRowsProducer);
+          ok = false;
+          break;
+        }
+        uint8_t* sx = tiles + s * stage_bytes;
+        mbar_arrive_expect_tx(&full[s], (x_rows + 2 * width) * 128);
+        tma_load_2d(sx, tmap_x, &full[s], it * BK, 0);
+        tma_load_2d(sx + kATileBytes, tmap_w, &full[s], it * BK, col0);
+        tma_load_2d(sx + kATileBytes + width * 128, tmap_w, &full[s], it * BK, p.F + col0);
+      }
+      if (!ok) {
+        // let the copies still in flight land before this CTA's shared memory is given up
+        for (int i = it > stages ? it - stages : 0; i < it; ++i)
+          if (!mbar_wait(&full[i % stages], (i / stages) & 1, p.wait_ns)) gated_report(p, kTimeoutRowsDrain);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc_f16(true, false, false, BM, 2 * width);
+      bool ok = true;
+      for (int it = 0; it < kblocks; ++it) {
+        const int s = it % stages;
+        if (!mbar_wait(&full[s], (it / stages) & 1, p.wait_ns)) {
+          gated_report(p, kTimeoutRowsMma);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t sx = smem_u32(tiles + s * stage_bytes), sw = sx + kATileBytes;
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k)
+          tc_mma_f16(tmem_base, make_smem_desc(sx + k * 32, 0, 1024), make_smem_desc(sw + k * 32, 0, 1024), idesc, (it | k) != 0);
+        tc_commit(&empty[s]);
+      }
+      if (ok) tc_commit(acc_full);
+    }
+  } else {
+    const int q = warp & 3;
+    if (q * 32 < p.T) {
+      if (mbar_wait(acc_full, 0, p.wait_ns)) {
+        tc_fence_after_sync();
+        // every product is done, so the stages are free to be the epilogue's patches
+        gated_epilogue<kAct, kSave>(p, tmem_base + ((uint32_t)(q * 32) << 16), width, width, tiles + q * kPatchBytes, lane, q * 32, col0);
+      } else if (lane == 0) {
+        gated_report(p, kTimeoutRowsEpilogue);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  body_sync();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, kRowsTmemCols);
+  }
+}
+
 }  // namespace gated
 }  // namespace mb
