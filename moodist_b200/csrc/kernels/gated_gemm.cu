@@ -8,6 +8,8 @@
 namespace mb {
 namespace gemm {
 int make_tmap_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
+int make_tmap_bf16_stack(CUtensorMap* out, const void* base, uint64_t count, uint64_t apart, uint64_t rows, uint64_t cols, uint64_t ld,
+                         uint32_t box_rows);
 }
 namespace gated {
 
@@ -56,14 +58,14 @@ static int launch_pair(GatedParams& p, const CUtensorMap& tx, const CUtensorMap&
 
 template <int kAct, bool kSave>
 __global__ void __launch_bounds__(kNumThreads, 1)
-    gated_rows_kernel(const __grid_constant__ GatedParams p, int width, int x_rows, const __grid_constant__ CUtensorMap tmap_x,
+    gated_rows_kernel(const __grid_constant__ GatedParams p, int width, int n, int split, const __grid_constant__ CUtensorMap tmap_x,
                       const __grid_constant__ CUtensorMap tmap_w) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  gated_rows_body<kAct, kSave>(p, width, x_rows, &tmap_x, &tmap_w, smem_raw);
+  gated_rows_body<kAct, kSave>(p, width, n, split, &tmap_x, &tmap_w, smem_raw);
 }
 
 template <int kAct, bool kSave>
-static int launch_rows(const GatedParams& p, int width, int x_rows, const CUtensorMap& tx, const CUtensorMap& tw, int device,
+static int launch_rows(const GatedParams& p, int width, int n, int split, const CUtensorMap& tx, const CUtensorMap& tw, int device,
                        cudaStream_t stream) {
   auto kern = gated_rows_kernel<kAct, kSave>;
   static bool configured[kMaxDevices];  // per instantiation
@@ -71,22 +73,40 @@ static int launch_rows(const GatedParams& p, int width, int x_rows, const CUtens
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) != cudaSuccess) return MB_ERR_LAUNCH;
     configured[device] = true;
   }
-  kern<<<(p.F + width - 1) / width, kNumThreads, kRowsSmem, stream>>>(p, width, x_rows, tx, tw);
-  return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((p.F + width - 1) / width * split, 1, 1);
+  cfg.blockDim = dim3(kNumThreads, 1, 1);
+  cfg.dynamicSmemBytes = kRowsSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p, width, n, split, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
-// Columns of h per CTA in the few-rows kernel: the narrowest multiple of 8 with which as few waves as 128 columns would
-// need cover F.
-static int rows_width(int F, int device) {
+// Columns of h per CTA and CTAs per K range of the few-rows kernel. One wave of CTAs is to cover F with the narrowest width
+// (a multiple of 8) that does; from 128 SMs' worth of columns up it takes more waves. Where F is so small that tiles of 64
+// columns leave SMs over, up to 8 CTAs split K, as long as each keeps 8 steps of 64. Clusters of several CTAs do not fill
+// every SM, so a sixteenth of them is not counted on then.
+static void rows_shape(int F, int K, int device, int& width, int& split) {
   static int sms[kMaxDevices];
   if (sms[device] == 0) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
     sms[device] = n;
   }
+  for (split = 8; split > 1; split /= 2) {
+    const int tiles = (sms[device] - sms[device] / 16) / split;
+    width = ((F + tiles - 1) / tiles + 7) / 8 * 8;
+    if (width <= 64 && K >= split * 8 * BK) return;
+  }
   const int waves = (F + 128 * sms[device] - 1) / (128 * sms[device]);
   const int ctas = waves * sms[device];
-  return ((F + ctas - 1) / ctas + 7) / 8 * 8;
+  width = ((F + ctas - 1) / ctas + 7) / 8 * 8;
 }
 
 // dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F], bound by their bytes.
@@ -132,11 +152,14 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   // Few rows: the weight's bytes bound the time and a 256-row tile would leave SMs idle (one token, F = 14336, K = 4096:
   // 65 us in pair tiles).
   const bool few = T <= BM;
-  const int width = few ? rows_width(F, device) : kHCols, x_rows = few ? (int)(T + 7) / 8 * 8 : BM;
+  int width = kHCols, split = 1;
+  if (few) rows_shape(F, K, device, width, split);
+  const int x_rows = few ? (int)(T + 15) / 16 * 16 : BM;
   CUtensorMap tx, tw;
   int rc = gemm::make_tmap_bf16(&tx, x, T, K, ldx, x_rows);
   if (rc) return rc;
-  rc = gemm::make_tmap_bf16(&tw, w, 2 * (uint64_t)F, K, ldw, width);
+  rc = few ? gemm::make_tmap_bf16_stack(&tw, w, 2, F * (uint64_t)ldw, F, K, ldw, width)
+           : gemm::make_tmap_bf16(&tw, w, 2 * (uint64_t)F, K, ldw, width);
   if (rc) return rc;
   GatedParams p{};
   p.T = (int)T;
@@ -153,12 +176,12 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   p.wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
   cudaStream_t s = MB_STREAM(stream);
   switch (act * 2 + (gu ? 1 : 0)) {
-    case 0: return few ? launch_rows<kSilu, false>(p, width, x_rows, tx, tw, device, s) : launch_pair<kSilu, false>(p, tx, tw, device, s);
-    case 1: return few ? launch_rows<kSilu, true>(p, width, x_rows, tx, tw, device, s) : launch_pair<kSilu, true>(p, tx, tw, device, s);
-    case 2: return few ? launch_rows<kGelu, false>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGelu, false>(p, tx, tw, device, s);
-    case 3: return few ? launch_rows<kGelu, true>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGelu, true>(p, tx, tw, device, s);
-    case 4: return few ? launch_rows<kGeluTanh, false>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGeluTanh, false>(p, tx, tw, device, s);
-    default: return few ? launch_rows<kGeluTanh, true>(p, width, x_rows, tx, tw, device, s) : launch_pair<kGeluTanh, true>(p, tx, tw, device, s);
+    case 0: return few ? launch_rows<kSilu, false>(p, width, x_rows, split, tx, tw, device, s) : launch_pair<kSilu, false>(p, tx, tw, device, s);
+    case 1: return few ? launch_rows<kSilu, true>(p, width, x_rows, split, tx, tw, device, s) : launch_pair<kSilu, true>(p, tx, tw, device, s);
+    case 2: return few ? launch_rows<kGelu, false>(p, width, x_rows, split, tx, tw, device, s) : launch_pair<kGelu, false>(p, tx, tw, device, s);
+    case 3: return few ? launch_rows<kGelu, true>(p, width, x_rows, split, tx, tw, device, s) : launch_pair<kGelu, true>(p, tx, tw, device, s);
+    case 4: return few ? launch_rows<kGeluTanh, false>(p, width, x_rows, split, tx, tw, device, s) : launch_pair<kGeluTanh, false>(p, tx, tw, device, s);
+    default: return few ? launch_rows<kGeluTanh, true>(p, width, x_rows, split, tx, tw, device, s) : launch_pair<kGeluTanh, true>(p, tx, tw, device, s);
   }
 }
 

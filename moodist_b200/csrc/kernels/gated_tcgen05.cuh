@@ -14,6 +14,7 @@
 #pragma once
 
 #include "gemm_pair_tcgen05.cuh"
+#include "vec_io.cuh"
 
 namespace mb {
 namespace gated {
@@ -161,7 +162,7 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
   volatile uint32_t* abort_flag = tmem_base_slot + 1;
   uint8_t* epi_patch = reinterpret_cast<uint8_t*>(bars) + 256;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const int cta_rank = (int)cluster_ctarank();  // 0 = leader
   const int num_tiles = p.tiles_m * p.tiles_n;
   const int kblocks = (p.K + BK - 1) / BK;
@@ -193,7 +194,7 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
   const uint32_t tmem_base = *tmem_base_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += stride) {
@@ -218,7 +219,7 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
       if (!ok) *abort_flag = 1;
     }
   } else if (warp == 1) {
-    if (lane == 0 && cta_rank == 0) {
+    if (cta_rank == 0 && elect_one()) {
       constexpr uint32_t idesc = make_idesc_f16(true, false, false, kPairBM, BN);
       uint32_t it = 0, local_tile = 0;
       bool ok = true;
@@ -288,40 +289,59 @@ __device__ __forceinline__ void gated_pair_body(const GatedParams& p, const CUte
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
 // Up to 128 rows the weight's bytes are the bound (4 F K of them: 36 us at F = 14336, K = 4096 and the measured copy rate),
-// and a 256-row tile leaves most SMs without one. Here a single CTA computes all rows of `width` columns of h, with the width
-// chosen so that one wave of CTAs covers F; 128 x 2 width accumulators, gate columns first. Only the rows of x that exist
-// are loaded (rounded up to 8): the tensor core reads what lies in the other rows of the 128-row operand, whose results
-// nothing looks at.
+// and a 256-row tile leaves most SMs without one. Here the weight is the M operand: a CTA computes `width` columns of h for
+// all rows, the width chosen so that one wave of CTAs covers F, from 128 weight rows by n >= T rows of x per product.
+//   width <= 64: gate and up rows are the two halves of one M tile, and the `split` CTAs of a cluster may share the K steps;
+//                they join their sums through distributed shared memory, in rank order
+//   width <= 128: two products per step, gate and up, which share the step's x
+// A stage holds exactly the rows that exist (2 width of the weight, n of x), so nearly all of shared memory is weight in
+// flight. The tensor core reads 128 rows from each operand's start all the same: those past the width are whatever the stage
+// and its successor hold, in rows of the accumulators that nothing looks at; kRowsSlack keeps the last stage's inside the
+// allocation.
+// Each CTA begins its K range elsewhere and wraps around: in step, all of them would ask for the same few lines of x at
+// the same time, which L2 serves one after the other (0.35 us a step whatever the width).
 enum RowsStatus : uint32_t {
   kTimeoutRowsProducer = 0x131,
   kTimeoutRowsMma = 0x132,
   kTimeoutRowsEpilogue = 0x133,
   kTimeoutRowsDrain = 0x134,
 };
-constexpr int kRowsMaxStages = 8;
+constexpr int kRowsMaxStages = 32;
 constexpr int kRowsSmem = 227 * 1024;
-constexpr int kRowsTmemCols = 256;
+constexpr int kRowsSlack = (BM - 8) * 128;
+constexpr int kRowsBars = (2 * kRowsMaxStages + 1) * 8 + 8;
 
-__host__ __device__ inline int rows_stage_bytes(int width) { return kATileBytes + 2 * width * 128; }
-__host__ __device__ inline int rows_stages(int width) {
-  const int n = (kRowsSmem - 1024 - 256) / rows_stage_bytes(width);
-  return n < kRowsMaxStages ? n : kRowsMaxStages;
+__host__ __device__ inline int rows_stage_bytes(int width, int n) { return (2 * width + n) * 128; }
+__host__ __device__ inline int rows_stages(int width, int n) {
+  const int fit = (kRowsSmem - 1024 - kRowsSlack - kRowsBars) / rows_stage_bytes(width, n);
+  return fit < kRowsMaxStages ? fit : kRowsMaxStages;
+}
+
+// four floats of the shared memory of any CTA of this cluster (a shared::cluster address; a local one is one too)
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 
 template <int kAct, bool kSave>
-__device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width, int x_rows, const CUtensorMap* tmap_x,
+__device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width, int n, int split, const CUtensorMap* tmap_x,
                                                 const CUtensorMap* tmap_w, uint8_t* smem_raw) {
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* tiles = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
-  const int stages = rows_stages(width), stage_bytes = rows_stage_bytes(width);
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);  // [stages]
-  uint64_t* empty = full + kRowsMaxStages;                                     // [stages]
+  const int stages = rows_stages(width, n), stage_bytes = rows_stage_bytes(width, n);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes + kRowsSlack);  // [stages]
+  uint64_t* empty = full + kRowsMaxStages;                                                  // [stages]
   uint64_t* acc_full = empty + kRowsMaxStages;
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kblocks = (p.K + BK - 1) / BK;
-  const int col0 = blockIdx.x * width;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const bool one_tile = 2 * width <= BM;
+  const int rank = blockIdx.x % split, tile = blockIdx.x / split, col0 = tile * width;
+  const int all_steps = (p.K + BK - 1) / BK;
+  const int step0 = (int)((int64_t)all_steps * rank / split), steps = (int)((int64_t)all_steps * (rank + 1) / split) - step0;
+  const int columns = one_tile ? n : 2 * n;
+  const uint32_t tmem_cols = columns <= 32 ? 32 : columns <= 64 ? 64 : columns <= 128 ? 128 : 256;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
@@ -335,7 +355,7 @@ __device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width,
     tma_prefetch_desc(tmap_w);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_base_slot, kRowsTmemCols);
+    tmem_alloc(tmem_base_slot, tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -343,22 +363,31 @@ __device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width,
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_base_slot;
 
+  // Stage index, phase and operand addresses are carried along: with one thread issuing copies and one issuing products, the
+  // instructions between two of them count.
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
-      int it = 0;
-      for (; it < kblocks; ++it) {
-        const int s = it % stages;
-        if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, p.wait_ns)) {
+      int it = 0, s = 0, at = (int)((int64_t)steps * tile * split / gridDim.x);
+      uint32_t phase = 1;
+      uint8_t* sw = tiles;
+      for (; it < steps; ++it) {
+        if (!mbar_wait(&empty[s], phase, p.wait_ns)) {
           gated_report(p, kTimeoutRowsProducer);
           ok = false;
           break;
         }
-        uint8_t* sx = tiles + s * stage_bytes;
-        mbar_arrive_expect_tx(&full[s], (x_rows + 2 * width) * 128);
-        tma_load_2d(sx, tmap_x, &full[s], it * BK, 0);
-        tma_load_2d(sx + kATileBytes, tmap_w, &full[s], it * BK, col0);
-        tma_load_2d(sx + kATileBytes + width * 128, tmap_w, &full[s], it * BK, p.F + col0);
+        const int k0 = (step0 + at) * BK;
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        tma_load_3d(sw, tmap_w, &full[s], k0, col0, 0);  // gate rows, then up rows
+        tma_load_2d(sw + 2 * width * 128, tmap_x, &full[s], k0, 0);
+        if (++at == steps) at = 0;
+        sw += stage_bytes;
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1;
+          sw = tiles;
+        }
       }
       if (!ok) {
         // let the copies still in flight land before this CTA's shared memory is given up
@@ -367,42 +396,97 @@ __device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width,
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = make_idesc_f16(true, false, false, BM, 2 * width);
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc_f16(true, false, false, BM, n);
+      const uint64_t first = make_smem_desc(smem_u32(tiles), 0, 1024);
+      const uint32_t to_up = (width * 128) >> 4, to_x = 2 * to_up;
       bool ok = true;
-      for (int it = 0; it < kblocks; ++it) {
-        const int s = it % stages;
-        if (!mbar_wait(&full[s], (it / stages) & 1, p.wait_ns)) {
+      int s = 0;
+      uint32_t phase = 0;
+      uint64_t dg = first;
+      for (int it = 0; it < steps; ++it) {
+        if (!mbar_wait(&full[s], phase, p.wait_ns)) {
           gated_report(p, kTimeoutRowsMma);
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        const uint32_t sx = smem_u32(tiles + s * stage_bytes), sw = sx + kATileBytes;
 #pragma unroll
-        for (int k = 0; k < BK / UMMA_K; ++k)
-          tc_mma_f16(tmem_base, make_smem_desc(sx + k * 32, 0, 1024), make_smem_desc(sw + k * 32, 0, 1024), idesc, (it | k) != 0);
+        for (int k = 0; k < BK / UMMA_K; ++k) {
+          tc_mma_f16(tmem_base, dg + k * 2, dg + to_x + k * 2, idesc, it | k);
+          if (!one_tile) tc_mma_f16(tmem_base + n, dg + to_up + k * 2, dg + to_x + k * 2, idesc, it | k);
+        }
         tc_commit(&empty[s]);
+        dg += stage_bytes >> 4;
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1;
+          dg = first;
+        }
       }
       if (ok) tc_commit(acc_full);
     }
   } else {
-    const int q = warp & 3;
-    if (q * 32 < p.T) {
-      if (mbar_wait(acc_full, 0, p.wait_ns)) {
-        tc_fence_after_sync();
-        // every product is done, so the stages are free to be the epilogue's patches
-        gated_epilogue<kAct, kSave>(p, tmem_base + ((uint32_t)(q * 32) << 16), width, width, tiles + q * kPatchBytes, lane, q * 32, col0);
-      } else if (lane == 0) {
-        gated_report(p, kTimeoutRowsEpilogue);
+    // Accumulators to shared memory as sums[row of x][gate columns, up columns] in fp32: every product is done, so the stages
+    // are free (2 width x T floats are never more than they hold).
+    const int q = warp & 3, r = q * 32 + lane;
+    float* sums = reinterpret_cast<float*>(tiles);
+    if (mbar_wait(acc_full, 0, p.wait_ns)) {
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+      const int held = one_tile ? 2 * width : width;
+#pragma unroll 1
+      for (int c = 0; c < columns && q * 32 < held; c += 16) {
+        uint32_t v[16];
+        tmem_ld_32x16(taddr + c, v);
+        tmem_ld_wait();
+        const int row0 = c < n ? c : c - n;
+        float* to = sums + row0 * 2 * width + (c < n ? 0 : width) + r;
+        if (r < held) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (row0 + i < p.T) to[i * 2 * width] = __uint_as_float(v[i]);
+        }
       }
+    } else if (lane == 0) {
+      gated_report(p, kTimeoutRowsEpilogue);
+    }
+    tc_fence_before_sync();
+  }
+  body_sync();
+  if (split > 1) cluster_sync_all();  // every CTA of the cluster has its sums in place
+  // each CTA of the cluster finishes its share of the (row, 8 columns) pieces
+  {
+    const int vecs = width / 8, pieces = p.T * vecs;
+    const uint32_t here = smem_u32(tiles);
+    for (int i = rank * kNumThreads + (int)threadIdx.x; i < pieces; i += split * kNumThreads) {
+      const int t = i / vecs, j = (i - t * vecs) * 8, col = col0 + j;
+      if (col >= p.F) continue;
+      float g[8], u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = u[k] = 0.f;
+      for (int c = 0; c < split; ++c) {
+        const uint32_t from = (split > 1 ? map_to_cta(here, c) : here) + (t * 2 * width + j) * 4;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float4 a = ld_cluster_f4(from + k * 16), b = ld_cluster_f4(from + width * 4 + k * 16);
+          g[4 * k] += a.x, g[4 * k + 1] += a.y, g[4 * k + 2] += a.z, g[4 * k + 3] += a.w;
+          u[4 * k] += b.x, u[4 * k + 1] += b.y, u[4 * k + 2] += b.z, u[4 * k + 3] += b.w;
+        }
+      }
+      if (kSave) {
+        store_vec<__nv_bfloat16, 8>(p.gu + t * p.ldgu + col, g);
+        store_vec<__nv_bfloat16, 8>(p.gu + t * p.ldgu + p.F + col, u);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = activate<kAct>(g[k]) * u[k];
+      store_vec<__nv_bfloat16, 8>(p.h + t * p.ldh + col, g);
     }
   }
-  tc_fence_before_sync();
-  body_sync();
+  if (split > 1) cluster_sync_all();  // the peers no longer read this CTA's sums
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, kRowsTmemCols);
+    tmem_dealloc(tmem_base, tmem_cols);
   }
 }
 

@@ -53,6 +53,24 @@ int make_tmap_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t c
   return r == CUDA_SUCCESS ? MB_OK : MB_ERR_DRIVER;
 }
 
+// The same over `count` row-major matrices of [rows, cols], `apart` elements from one to the next; a box takes box_rows of each
+// (count x box_rows rows of shared memory).
+int make_tmap_bf16_stack(CUtensorMap* out, const void* base, uint64_t count, uint64_t apart, uint64_t rows, uint64_t cols, uint64_t ld,
+                         uint32_t box_rows) {
+  EncodeFn enc = get_encode();
+  ensure_context();
+  if (!enc) return MB_ERR_DRIVER;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((ld * 2) & 15) || ((apart * 2) & 15)) return MB_ERR_ALIGN;
+  cuuint64_t dims[3] = {cols, rows, count};
+  cuuint64_t strides[2] = {ld * 2, apart * 2};
+  cuuint32_t box[3] = {64, box_rows, (cuuint32_t)count};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MB_OK : MB_ERR_DRIVER;
+}
+
 template <bool kAMn, bool kBMn, typename OutT>
 __global__ void __launch_bounds__(kNumThreads, 1)
     gemm_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap tmap_a,
