@@ -74,7 +74,7 @@ static int launch_rows(const GatedParams& p, int width, int n, int split, const 
     configured[device] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = split;
   attr[0].val.clusterDim.y = 1;
@@ -84,7 +84,9 @@ static int launch_rows(const GatedParams& p, int width, int n, int split, const 
   cfg.dynamicSmemBytes = kRowsSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, p, width, n, split, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 

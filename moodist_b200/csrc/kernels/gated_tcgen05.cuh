@@ -362,6 +362,8 @@ __device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width,
   body_sync();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_base_slot;
+  grid_wait();
+  grid_release();
 
   // Stage index, phase and operand addresses are carried along: with one thread issuing copies and one issuing products, the
   // instructions between two of them count.

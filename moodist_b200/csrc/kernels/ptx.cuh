@@ -207,6 +207,12 @@ __device__ __forceinline__ bool elect_one() {
 // threadIdx.x / 32 as a value the assembler knows to be the same in the whole warp
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
+// Programmatic dependent launch: a kernel launched with that attribute may begin while the one before it in the stream
+// drains; grid_wait returns once that one's results are in memory (at once without the attribute), grid_release lets the
+// next one begin.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------------------
 // TMA: tiled loads from THIS GPU's memory into this CTA's shared memory (no cluster multicast)
 // ---------------------------------------------------------------------------------------------
