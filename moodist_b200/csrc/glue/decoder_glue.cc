@@ -135,7 +135,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                          dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
                          db.defined() ? db.data_ptr() : nullptr, partial.defined() ? partial.data_ptr<float>() : nullptr, rows,
                          D, x2.stride(0), dy.stride(0), D, dtype_code(x2.scalar_type()), w_code, cur_stream()),
-        wants[0] + 2 * (wants[1] || wants[2]), "layer_norm backward");
+        1 + (wants[1] || wants[2]), "layer_norm backward");
     return {dx, dw, db, at::Tensor()};
   }
 };

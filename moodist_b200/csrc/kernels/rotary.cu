@@ -82,11 +82,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p) {
           o[k + V] = ob;
         }
       }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        va.v[k] = from_f32<T>(o[k]);
-        vb.v[k] = from_f32<T>(o[k + V]);
-      }
+      va = pack<T, V>(o);
+      vb = pack<T, V>(o + V);
     }
     *reinterpret_cast<Pack<T, V>*>(out + first) = va;
     *reinterpret_cast<Pack<T, V>*>(out + second) = vb;
