@@ -4,8 +4,9 @@
 //   a' = a c - b s,  b' = b c + a s      (c, s) = (cos, sin)[position, j];  the backward pass takes -s (the transpose)
 //   half layout:  pairs (j, j + R/2);    interleaved: pairs (2j, 2j + 1)
 //
-// Bound by the bytes of q and k, read once and written once. A thread moves V elements of both members of V pairs with two
-// vector loads and two vector stores, V * sizeof(T) = 16 bytes where sizes, strides and addresses allow.
+// Bound by the bytes of q and k, read once and written once. A thread takes V pairs of one token (V * sizeof(T) = 16 bytes where
+// sizes, strides and addresses allow: two vector loads and two vector stores) in four neighbouring heads: eight loads in
+// flight, and the cosines and sines, which are twice the bytes of the pairs of one 16-bit head, are read once for the four.
 #include "kernels_api.h"
 #include "vec_io.cuh"
 
@@ -17,76 +18,111 @@ using namespace mb;
 
 inline int check_launch() { return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH; }
 
+constexpr int kHeads = 4;  // heads per thread
+
 template <typename T, int V>
-__global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p) {
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+
+template <typename T, int V, bool kInterleaved>
+__global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p, int64_t threads) {
   const int half = p.rot / 2;
-  const int turns = half / V;                                  // items of a head that turn
-  const int copies = (p.dim - p.rot + 2 * V - 1) / (2 * V);    // items that only move (none in place)
-  const int per_head = turns + (p.in_place ? 0 : copies);
-  const int heads = p.q_heads + p.k_heads;
-  const int64_t total = p.batch * p.seq * heads * per_head;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int item = (int)(i % per_head);
-    int64_t rest = i / per_head;
-    int h = (int)(rest % heads);
-    rest /= heads;
-    const int64_t s = rest % p.seq, b = rest / p.seq;
-    const bool is_k = h >= p.q_heads;
-    if (is_k) h -= p.q_heads;
-    const mb_rotary_heads_t& x = is_k ? p.k : p.q;
-    const T* in = reinterpret_cast<const T*>(x.in) + b * x.in_batch + s * x.in_seq + h * x.in_head;
-    T* out = reinterpret_cast<T*>(x.out) + b * x.out_batch + s * x.out_seq + h * x.out_head;
-    if (item >= turns) {
-      const int c = p.rot + (item - turns) * 2 * V;
+  const int turns = half / V;                                                      // items of a head that turn
+  const int copies = p.in_place ? 0 : (p.dim - p.rot + 2 * V - 1) / (2 * V);       // items that only move
+  const int per_head = turns + copies, heads = p.q_heads + p.k_heads;
+  const int chunks = (heads + kHeads - 1) / kHeads;
+  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= threads) return;
+  int64_t b, s;
+  int chunk, item;
+  if (threads <= 0xffffffffll) {
+    const uint32_t u = (uint32_t)i, q = u / (uint32_t)per_head, t = q / (uint32_t)chunks, bb = t / (uint32_t)p.seq;
+    item = (int)(u - q * per_head);
+    chunk = (int)(q - t * chunks);
+    b = bb;
+    s = t - bb * (uint32_t)p.seq;
+  } else {
+    const int64_t q = i / per_head;
+    item = (int)(i - q * per_head);
+    const int64_t token = q / chunks;
+    chunk = (int)(q - token * chunks);
+    b = token / p.seq;
+    s = token - b * p.seq;
+  }
+  const int h0 = chunk * kHeads;
+  const T* in[kHeads];
+  T* out[kHeads];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (c + k * V < p.dim)
-          *reinterpret_cast<Pack<T, V>*>(out + c + k * V) = *reinterpret_cast<const Pack<T, V>*>(in + c + k * V);
-      continue;
+  for (int k = 0; k < kHeads; ++k) {
+    const bool is_k = h0 + k >= p.q_heads;
+    const mb_rotary_heads_t& x = is_k ? p.k : p.q;
+    const int64_t h = is_k ? h0 + k - p.q_heads : h0 + k;
+    in[k] = reinterpret_cast<const T*>(x.in) + b * x.in_batch + s * x.in_seq + h * x.in_head;
+    out[k] = reinterpret_cast<T*>(x.out) + b * x.out_batch + s * x.out_seq + h * x.out_head;
+  }
+  const int j = item * V;
+  const bool moves = item >= turns;
+  const int rest = p.rot + 2 * (j - half);
+  const int first = moves ? rest : kInterleaved ? 2 * j : j;
+  const int second = moves ? rest + V : kInterleaved ? 2 * j + V : j + half;
+  const bool both = !moves || second < p.dim;
+  Pack<T, V> va[kHeads], vb[kHeads];
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    if (h0 + k < heads) {
+      va[k] = load_pack<T, V>(in[k] + first);
+      if (both) vb[k] = load_pack<T, V>(in[k] + second);
     }
+  }
+  if (!moves) {
     int64_t pos = s;
     if (p.positions) {
       const int64_t at = b * p.pos_batch + s * p.pos_seq;
       pos = p.pos_i64 ? reinterpret_cast<const int64_t*>(p.positions)[at] : reinterpret_cast<const int32_t*>(p.positions)[at];
     }
-    const int j = item * V;
-    const int first = p.interleaved ? 2 * j : j, second = p.interleaved ? 2 * j + V : j + half;
-    Pack<T, V> va = *reinterpret_cast<const Pack<T, V>*>(in + first);
-    Pack<T, V> vb = *reinterpret_cast<const Pack<T, V>*>(in + second);
     if (pos >= p.length) {
       // a position that the tables do not have shows as NaN
+      float nan[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) va.v[k] = vb.v[k] = from_f32<T>(NAN);
+      for (int e = 0; e < V; ++e) nan[e] = NAN;
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) va[k] = vb[k] = pack<T, V>(nan);
     } else if (pos >= 0) {
+      constexpr int kStep = V <= 4 ? V : 4;
       float c[V], sn[V];
-      load_vec<float, V <= 4 ? V : 4>(p.cos_tab + pos * half + j, c);
-      load_vec<float, V <= 4 ? V : 4>(p.sin_tab + pos * half + j, sn);
-      if (V == 8) {
-        load_vec<float, 4>(p.cos_tab + pos * half + j + 4, c + V / 2);
-        load_vec<float, 4>(p.sin_tab + pos * half + j + 4, sn + V / 2);
-      }
-      float f[2 * V], o[2 * V];
-      unpack<T, V>(va, f);
-      unpack<T, V>(vb, f + V);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float sk = p.inverse ? -sn[k] : sn[k];
-        const float a = p.interleaved ? f[2 * k] : f[k], bb = p.interleaved ? f[2 * k + 1] : f[k + V];
-        // spelled out, so that every vector width gives the same bits
-        const float oa = fmaf(a, c[k], -__fmul_rn(bb, sk)), ob = fmaf(bb, c[k], __fmul_rn(a, sk));
-        if (p.interleaved) {
-          o[2 * k] = oa;
-          o[2 * k + 1] = ob;
-        } else {
-          o[k] = oa;
-          o[k + V] = ob;
-        }
+      for (int e = 0; e < V; e += kStep) {
+        load_vec<float, kStep>(p.cos_tab + pos * half + j + e, c + e);
+        load_vec<float, kStep>(p.sin_tab + pos * half + j + e, sn + e);
       }
-      va = pack<T, V>(o);
-      vb = pack<T, V>(o + V);
+      if (p.inverse) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) sn[e] = -sn[e];
+      }
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        float f[2 * V], o[2 * V];
+        unpack<T, V>(va[k], f);
+        unpack<T, V>(vb[k], f + V);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int ia = kInterleaved ? 2 * e : e, ib = kInterleaved ? 2 * e + 1 : e + V;
+          // spelled out, so that every vector width gives the same bits
+          o[ia] = fmaf(f[ia], c[e], -__fmul_rn(f[ib], sn[e]));
+          o[ib] = fmaf(f[ib], c[e], __fmul_rn(f[ia], sn[e]));
+        }
+        va[k] = pack<T, V>(o);
+        vb[k] = pack<T, V>(o + V);
+      }
     }
-    *reinterpret_cast<Pack<T, V>*>(out + first) = va;
-    *reinterpret_cast<Pack<T, V>*>(out + second) = vb;
+  }
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    if (h0 + k < heads) {
+      *reinterpret_cast<Pack<T, V>*>(out[k] + first) = va[k];
+      if (both) *reinterpret_cast<Pack<T, V>*>(out[k] + second) = vb[k];
+    }
   }
 }
 
@@ -100,11 +136,14 @@ bool fits(const mb_rotary_heads_t& x, int heads, int V, int elem) {
 template <typename T, int V>
 int launch(const mb_rotary_t& p, cudaStream_t stream) {
   const int64_t per_head = p.rot / 2 / V + (p.in_place ? 0 : (p.dim - p.rot + 2 * V - 1) / (2 * V));
-  const int64_t items = p.batch * p.seq * (p.q_heads + p.k_heads) * per_head;
-  if (items == 0) return MB_OK;
-  int64_t grid = (items + 255) / 256;
-  if (grid > 148 * 16) grid = 148 * 16;
-  rotary_kernel<T, V><<<(unsigned)grid, 256, 0, stream>>>(p);
+  const int64_t threads = p.batch * p.seq * ((p.q_heads + p.k_heads + kHeads - 1) / kHeads) * per_head;
+  if (threads == 0) return MB_OK;
+  const int64_t grid = (threads + 255) / 256;
+  if (grid > 0x7fffffffll) return MB_ERR_TOO_BIG;
+  if (p.interleaved)
+    rotary_kernel<T, V, true><<<(unsigned)grid, 256, 0, stream>>>(p, threads);
+  else
+    rotary_kernel<T, V, false><<<(unsigned)grid, 256, 0, stream>>>(p, threads);
   return check_launch();
 }
 
