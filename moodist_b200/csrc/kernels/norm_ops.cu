@@ -163,9 +163,7 @@ struct Held {
   __device__ __forceinline__ static int column(int t, int i) { return (i * kTpr + t) * kVec; }
   __device__ __forceinline__ void fill(float x) {
 #pragma unroll
-    for (int i = 0; i < kG; ++i)
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) v[i].v[k] = from_f32<T>(x);
+    for (int i = 0; i < kG; ++i) v[i] = splat<T, kVec>(x);
   }
   // columns from D up keep what they hold
   __device__ __forceinline__ void load(const T* row, int t, int D) {

@@ -25,13 +25,15 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
+// chunks of a tensor's heads
+__host__ __device__ __forceinline__ int head_chunks(int heads) { return (heads + kHeads - 1) / kHeads; }
+
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p, int64_t threads) {
+__global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ mb_rotary_t p, int64_t threads) {
   const int half = p.rot / 2;
-  const int turns = half / V;                                                      // items of a head that turn
-  const int copies = p.in_place ? 0 : (p.dim - p.rot + 2 * V - 1) / (2 * V);       // items that only move
-  const int per_head = turns + copies, heads = p.q_heads + p.k_heads;
-  const int chunks = (heads + kHeads - 1) / kHeads;
+  const int turns = half / V;                                                 // items of a head that turn
+  const int copies = p.in_place ? 0 : (p.dim - p.rot + 2 * V - 1) / (2 * V);  // items that only move
+  const int per_head = turns + copies, chunks = head_chunks(p.q_heads) + head_chunks(p.k_heads);
   const int64_t i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= threads) return;
   int64_t b, s;
@@ -50,29 +52,23 @@ __global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p, int64_
     b = token / p.seq;
     s = token - b * p.seq;
   }
-  const int h0 = chunk * kHeads;
-  const T* in[kHeads];
-  T* out[kHeads];
-#pragma unroll
-  for (int k = 0; k < kHeads; ++k) {
-    const bool is_k = h0 + k >= p.q_heads;
-    const mb_rotary_heads_t& x = is_k ? p.k : p.q;
-    const int64_t h = is_k ? h0 + k - p.q_heads : h0 + k;
-    in[k] = reinterpret_cast<const T*>(x.in) + b * x.in_batch + s * x.in_seq + h * x.in_head;
-    out[k] = reinterpret_cast<T*>(x.out) + b * x.out_batch + s * x.out_seq + h * x.out_head;
-  }
+  const bool is_k = chunk >= head_chunks(p.q_heads);
+  const mb_rotary_heads_t& x = is_k ? p.k : p.q;
+  const int h0 = (is_k ? chunk - head_chunks(p.q_heads) : chunk) * kHeads, heads = (is_k ? p.k_heads : p.q_heads) - h0;
   const int j = item * V;
   const bool moves = item >= turns;
   const int rest = p.rot + 2 * (j - half);
   const int first = moves ? rest : kInterleaved ? 2 * j : j;
-  const int second = moves ? rest + V : kInterleaved ? 2 * j + V : j + half;
-  const bool both = !moves || second < p.dim;
+  const int apart = moves || kInterleaved ? V : half;  // from the first vector to the second
+  const bool both = !moves || first + apart < p.dim;
+  const T* in = reinterpret_cast<const T*>(x.in) + b * x.in_batch + s * x.in_seq + h0 * x.in_head + first;
+  T* out = reinterpret_cast<T*>(x.out) + b * x.out_batch + s * x.out_seq + h0 * x.out_head + first;
   Pack<T, V> va[kHeads], vb[kHeads];
 #pragma unroll
   for (int k = 0; k < kHeads; ++k) {
-    if (h0 + k < heads) {
-      va[k] = load_pack<T, V>(in[k] + first);
-      if (both) vb[k] = load_pack<T, V>(in[k] + second);
+    if (k < heads) {
+      va[k] = load_pack<T, V>(in + k * x.in_head);
+      if (both) vb[k] = load_pack<T, V>(in + k * x.in_head + apart);
     }
   }
   if (!moves) {
@@ -83,11 +79,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p, int64_
     }
     if (pos >= p.length) {
       // a position that the tables do not have shows as NaN
-      float nan[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) nan[e] = NAN;
-#pragma unroll
-      for (int k = 0; k < kHeads; ++k) va[k] = vb[k] = pack<T, V>(nan);
+      for (int k = 0; k < kHeads; ++k) va[k] = vb[k] = splat<T, V>(NAN);
     } else if (pos >= 0) {
       constexpr int kStep = V <= 4 ? V : 4;
       float c[V], sn[V];
@@ -105,12 +98,25 @@ __global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p, int64_
         float f[2 * V], o[2 * V];
         unpack<T, V>(va[k], f);
         unpack<T, V>(vb[k], f + V);
+        // every vector width and layout rounds alike: first b s (a s), then its sum with a c (b c) in one step
+        if constexpr (kInterleaved || V == 1) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int ia = kInterleaved ? 2 * e : e, ib = kInterleaved ? 2 * e + 1 : e + V;
-          // spelled out, so that every vector width gives the same bits
-          o[ia] = fmaf(f[ia], c[e], -__fmul_rn(f[ib], sn[e]));
-          o[ib] = fmaf(f[ib], c[e], __fmul_rn(f[ia], sn[e]));
+          for (int e = 0; e < V; ++e) {
+            const int ia = kInterleaved ? 2 * e : e, ib = kInterleaved ? 2 * e + 1 : e + V;
+            const float2 t = split(fma2(f2(f[ia], f[ib]), f2(c[e]), mul2(f2(f[ib], f[ia]), f2(-sn[e], sn[e]))));
+            o[ia] = t.x;
+            o[ib] = t.y;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            const F2 a = f2(f[e], f[e + 1]), bb = f2(f[V + e], f[V + e + 1]), cc = f2(c[e], c[e + 1]), ss = f2(sn[e], sn[e + 1]);
+            const float2 ta = split(fma2(a, cc, mul2(bb, f2(-sn[e], -sn[e + 1])))), tb = split(fma2(bb, cc, mul2(a, ss)));
+            o[e] = ta.x;
+            o[e + 1] = ta.y;
+            o[V + e] = tb.x;
+            o[V + e + 1] = tb.y;
+          }
         }
         va[k] = pack<T, V>(o);
         vb[k] = pack<T, V>(o + V);
@@ -119,9 +125,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const mb_rotary_t p, int64_
   }
 #pragma unroll
   for (int k = 0; k < kHeads; ++k) {
-    if (h0 + k < heads) {
-      *reinterpret_cast<Pack<T, V>*>(out[k] + first) = va[k];
-      if (both) *reinterpret_cast<Pack<T, V>*>(out[k] + second) = vb[k];
+    if (k < heads) {
+      *reinterpret_cast<Pack<T, V>*>(out + k * x.out_head) = va[k];
+      if (both) *reinterpret_cast<Pack<T, V>*>(out + k * x.out_head + apart) = vb[k];
     }
   }
 }
@@ -136,7 +142,7 @@ bool fits(const mb_rotary_heads_t& x, int heads, int V, int elem) {
 template <typename T, int V>
 int launch(const mb_rotary_t& p, cudaStream_t stream) {
   const int64_t per_head = p.rot / 2 / V + (p.in_place ? 0 : (p.dim - p.rot + 2 * V - 1) / (2 * V));
-  const int64_t threads = p.batch * p.seq * ((p.q_heads + p.k_heads + kHeads - 1) / kHeads) * per_head;
+  const int64_t threads = p.batch * p.seq * (head_chunks(p.q_heads) + head_chunks(p.k_heads)) * per_head;
   if (threads == 0) return MB_OK;
   const int64_t grid = (threads + 255) / 256;
   if (grid > 0x7fffffffll) return MB_ERR_TOO_BIG;

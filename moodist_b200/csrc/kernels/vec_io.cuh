@@ -28,53 +28,79 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
   return __float2half_rn(v);
 }
 
-template <typename T, int N>
+// N elements as they lie in memory: 32-bit words (a struct of 16-bit members is taken apart and put together again member by
+// member in registers), or the single 16-bit element.
+template <typename T, int N, bool kWords = sizeof(T) * N % 4 == 0>
 struct alignas(sizeof(T) * N) Pack {
+  uint32_t w[sizeof(T) * N / 4];
+};
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack<T, N, false> {
   T v[N];
 };
 
-// Pairs are converted together: one instruction each way for two 16-bit values (single conversions to 16 bits run at a
+// Pairs are converted together: at most one instruction each way per 16-bit value (single conversions to 16 bits run at a
 // quarter of the rate, and made bf16 rows take as long as fp32 rows of twice the bytes).
-__device__ __forceinline__ float2 pair_to_f32(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-__device__ __forceinline__ float2 pair_to_f32(__half2 v) { return __half22float2(v); }
-__device__ __forceinline__ void pair_from_f32(float a, float b, __nv_bfloat162* v) { *v = __floats2bfloat162_rn(a, b); }
-__device__ __forceinline__ void pair_from_f32(float a, float b, __half2* v) { *v = __floats2half2_rn(a, b); }
 template <typename T>
-struct PairOf;
+__device__ __forceinline__ float2 pair_to_f32(uint32_t w);
 template <>
-struct PairOf<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-};
+__device__ __forceinline__ float2 pair_to_f32<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <>
-struct PairOf<__half> {
-  using type = __half2;
-};
+__device__ __forceinline__ float2 pair_to_f32<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_from_f32(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pair_from_f32<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pair_from_f32<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Pack<T, N>& p, float* f) {
-  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 v = pair_to_f32(*reinterpret_cast<const typename PairOf<T>::type*>(&p.v[i]));
-      f[i] = v.x;
-      f[i + 1] = v.y;
+    for (int i = 0; i < N; ++i) f[i] = __uint_as_float(p.w[i]);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 v = pair_to_f32<T>(p.w[i]);
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = to_f32(p.v[i]);
+    static_assert(N == 1, "one 16-bit element or pairs of them");
+    f[0] = to_f32(p.v[0]);
   }
 }
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> pack(const float* f) {
   Pack<T, N> p;
-  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) pair_from_f32(f[i], f[i + 1], reinterpret_cast<typename PairOf<T>::type*>(&p.v[i]));
+    for (int i = 0; i < N; ++i) p.w[i] = __float_as_uint(f[i]);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) p.w[i] = pair_from_f32<T>(f[2 * i], f[2 * i + 1]);
   } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) p.v[i] = from_f32<T>(f[i]);
+    p.v[0] = from_f32<T>(f[0]);
   }
   return p;
+}
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> splat(float x) {
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = x;
+  return pack<T, N>(f);
 }
 template <typename T, int N>
 __device__ __forceinline__ void load_vec(const T* p, float* f) {
