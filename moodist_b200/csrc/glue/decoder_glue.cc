@@ -343,10 +343,10 @@ mb_distill_t distill_args(const at::Tensor& z, const at::Tensor& ids, const at::
   d.hard = (float)hard;
   d.scale = (float)scale;
   d.mean = mean;
-  // one workspace: [1] factor, [rows] entropy, [rows, 3] stats, [rows] row losses, [rows] live, [rows, K] p
+  // one workspace: MB_DISTILL_COUNTS counts, [rows] entropy, [rows, 3] stats, [rows] row losses, [rows] live, [rows, K] p
   float* w = work.data_ptr<float>();
-  d.factor = w;
-  d.entropy = w + 1;
+  d.counts = reinterpret_cast<int*>(w);
+  d.entropy = w + MB_DISTILL_COUNTS;
   d.stats = d.entropy + rows;
   d.row_loss = d.stats + 3 * rows;
   d.live = reinterpret_cast<int*>(d.row_loss + rows);
@@ -359,16 +359,25 @@ struct Distill : torch::autograd::Function<Distill> {
                             const OptTensor& targets_opt, double tau, double hard, int64_t ignore_index, bool mean, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor targets_in = value(targets_opt);
+    const int64_t rows = logits.numel() / logits.size(-1), K = ids_in.size(-1);
+    if (!rows) {
+      if (ctx) ctx->saved_data["grad"] = at::empty(logits.sizes(), logits.options());
+      return at::zeros({}, logits.options().dtype(at::kFloat));
+    }
     at::Tensor z = as_rows(logits);
-    const int64_t rows = z.size(0), K = ids_in.size(-1);
     at::Tensor ids = ids_in.reshape({rows, K}).contiguous(), top = top_in.reshape({rows, K}).contiguous();
     at::Tensor targets = targets_in.defined() ? targets_in.reshape({rows}).contiguous() : targets_in;
-    at::Tensor work = at::empty({1 + rows * (6 + K)}, z.options().dtype(at::kFloat));
-    at::Tensor loss = at::empty({}, z.options().dtype(at::kFloat));
+    at::Tensor work = at::empty({MB_DISTILL_COUNTS + rows * (6 + K)}, z.options().dtype(at::kFloat));
+    at::Tensor loss = at::empty({}, z.options().dtype(at::kFloat)), dz;
     mb_distill_t d = distill_args(z, ids, top, targets, tau, hard, ignore_index, mean, scale, work);
     d.loss = loss.data_ptr<float>();
-    run(mb_distill_fwd(&d, cur_stream()), 4, "distill_loss");
-    if (ctx) {
+    // fp16 gradients wait for the incoming scale, which keeps them from underflowing
+    const bool now = ctx && logits.scalar_type() != at::kHalf;
+    if (now) dz = at::empty(logits.sizes(), logits.options());
+    run(mb_distill_fwd(&d, now ? dz.data_ptr() : nullptr, d.V, cur_stream()), 2, "distill_loss");
+    if (now) {
+      ctx->saved_data["grad"] = dz;
+    } else if (ctx) {
       ctx->save_for_backward({z, ids, top, targets, work});
       ctx->saved_data["shape"] = logits.sizes();
       ctx->saved_data["tau"] = tau;
@@ -384,12 +393,25 @@ struct Distill : torch::autograd::Function<Distill> {
     once("distill_loss");
     variable_list out(9);
     if (!grads[0].defined()) return out;
+    auto& a = ctx->saved_data;
+    at::Tensor g = grads[0].contiguous();
+    if (a.count("grad")) {
+      // the forward pass made the gradient; it is given away, and only scaled if the loss was
+      TORCH_CHECK(a["grad"].isTensor(), "moodist distill_loss: the gradient of this call has been taken already (a second backward pass "
+                  "through it needs a second forward pass)");
+      at::Tensor dz = a["grad"].toTensor();
+      a["grad"] = c10::IValue();
+      c10::cuda::CUDAGuard guard(dz.device());
+      run(mb_scale_by(dz.data_ptr(), dz.numel(), dtype_code(dz.scalar_type()), g.data_ptr<float>(), cur_stream()), 1,
+          "distill_loss backward");
+      out[0] = dz;
+      return out;
+    }
     const auto s = ctx->get_saved_variables();
     c10::cuda::CUDAGuard guard(s[0].device());
-    auto& a = ctx->saved_data;
     mb_distill_t d = distill_args(s[0], s[1], s[2], s[3], a["tau"].toDouble(), a["hard"].toDouble(), a["ignore"].toInt(),
                                   a["mean"].toBool(), a["scale"].toDouble(), s[4]);
-    at::Tensor g = grads[0].contiguous(), dz = at::empty(a["shape"].toIntVector(), s[0].options());
+    at::Tensor dz = at::empty(a["shape"].toIntVector(), s[0].options());
     run(mb_distill_bwd(&d, g.data_ptr<float>(), dz.data_ptr(), d.V, cur_stream()), 1, "distill_loss backward");
     out[0] = dz;
     return out;

@@ -4,7 +4,11 @@
 //   row   = (1 - hard) tau^2 sum_k p_k (log p_k - log q_{id_k}) + hard (logsumexp(z) - z_target)
 //   dz_j  = (1 - hard) tau (q_j - sum_{k: id_k = j} p_k) + hard (softmax(z)_j - [j = target])
 //
-// Bound by the bytes of the logits: read by the forward pass, read again and written as the gradient by the backward pass.
+// Bound by the bytes of the logits, read once, and of the gradient, written once. The gradient's scale is known in the forward
+// pass up to the incoming scalar (which is 1 unless the loss is scaled afterwards), so the forward pass writes it: a CTA walks a
+// row twice, first from memory for the maximum and the sum of exponentials, then for the gradient from L2, where the rows in
+// work (148 of 256 KB at 128256 words) stay. fp16 is the exception: its gradients would underflow before a loss scale reaches
+// them, so there the backward pass reads the logits again.
 // Sums and row statistics are fp32; sums have a fixed order, so the same inputs give the same bits.
 #include "kernels_api.h"
 #include "vec_io.cuh"
@@ -17,8 +21,11 @@ using namespace mb;
 
 inline int check_launch() { return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH; }
 
+constexpr int kSms = 148;
 constexpr int kTopThreads = 128;
-constexpr int kRowThreads = 512;
+constexpr int kTopCtas = kSms * 8;
+static_assert(kTopCtas + 1 <= MB_DISTILL_COUNTS, "one count per CTA and a ticket");
+constexpr int kStaged = 1024;  // teacher entries of a row that fit shared memory
 
 __device__ __forceinline__ int64_t id_at(const mb_distill_t& d, int64_t i) {
   return d.ids_i64 ? reinterpret_cast<const int64_t*>(d.ids)[i] : (int64_t)reinterpret_cast<const int32_t*>(d.ids)[i];
@@ -37,10 +44,12 @@ __device__ __forceinline__ bool entry(const mb_distill_t& d, int64_t i, float* t
   return *t != -INFINITY;
 }
 
-// One CTA per row: the teacher's probabilities over the valid entries (0 in the others), sum p log p, whether the row counts.
+// One CTA per row: the teacher's probabilities over the valid entries (0 in the others), sum p log p, whether the row counts;
+// per CTA how many rows do. Readies the ticket of the row kernel.
 __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const mb_distill_t d) {
   __shared__ float red[kTopThreads / 32];
   const float inv_tau = 1.f / d.tau;
+  int count = 0;
   for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
     const int64_t base = r * d.K;
     bool counts = true;
@@ -73,218 +82,432 @@ __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const mb_d
     const float inv = live ? 1.f / s : 0.f;
     for (int k = threadIdx.x; k < d.K; k += kTopThreads)
       d.p[base + k] = live && entry(d, base + k, &t) ? expf((t - m) * inv_tau) * inv : 0.f;
+    count += live;
     if (threadIdx.x == 0) {
       d.live[r] = live;
       d.entropy[r] = live ? e * inv - logf(s) : 0.f;
     }
   }
+  if (threadIdx.x == 0) {
+    d.counts[blockIdx.x] = count;
+    if (blockIdx.x == 0) d.counts[kTopCtas] = 0;
+  }
 }
 
-// factor = scale, or scale over the number of rows that count (one CTA)
-__global__ void __launch_bounds__(1024) distill_factor_kernel(const mb_distill_t d) {
-  __shared__ int part[32];
-  int n = 0;
-  for (int64_t r = threadIdx.x; r < d.rows; r += 1024) n += d.live[r];
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
+inline __host__ __device__ int top_ctas(int64_t rows) { return (int)(rows < kTopCtas ? rows : kTopCtas); }
+
+// scale, or scale over the number of rows that count; all threads of the CTA get it
+template <int kThreads>
+__device__ float row_factor(const mb_distill_t& d, int* shared) {
+  if (!d.mean) return d.scale;
+  if (threadIdx.x == 0) *shared = 0;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    n = __reduce_add_sync(0xffffffffu, part[threadIdx.x]);
-    if (threadIdx.x == 0) d.factor[0] = d.mean ? d.scale / (float)(n > 0 ? n : 1) : d.scale;
-  }
+  int n = 0;
+  for (int i = threadIdx.x; i < top_ctas(d.rows); i += kThreads) n += d.counts[i];
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) atomicAdd(shared, n);
+  __syncthreads();
+  return d.scale / (float)(*shared > 0 ? *shared : 1);
 }
 
-// one value joins a running maximum m and the sums of exp((z - m) / tau) and, with kHard, exp(z - m)
-template <bool kHard>
-__device__ __forceinline__ void join(float& m, float& st, float& s1, float om, float ost, float os1, float inv_tau) {
-  const float nm = fmaxf(m, om);
-  if (nm == -INFINITY) return;
-  const float a = m == -INFINITY ? 0.f : __expf((m - nm) * inv_tau), b = om == -INFINITY ? 0.f : __expf((om - nm) * inv_tau);
-  st = st * a + ost * b;
-  if (kHard) {
-    const float a1 = m == -INFINITY ? 0.f : __expf(m - nm), b1 = om == -INFINITY ? 0.f : __expf(om - nm);
-    s1 = s1 * a1 + os1 * b1;
-  }
-  m = nm;
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T, int kV, bool kHard>
-__global__ void __launch_bounds__(kRowThreads) distill_row_kernel(const mb_distill_t d) {
-  __shared__ float sm[3][kRowThreads / 32];
-  __shared__ float red[kRowThreads / 32];
-  const float inv_tau = 1.f / d.tau;
-  for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
-    if (!d.live[r]) {
-      if (threadIdx.x == 0) d.row_loss[r] = 0.f;
-      continue;
+// A row as single elements up to the first 16-byte boundary, vectors, and single elements behind the last.
+template <typename T>
+struct Row {
+  static constexpr int kV = 16 / sizeof(T);
+  int head, vecs, edge;  // edge: single elements at both ends together
+  __device__ __forceinline__ Row(const T* p, int V) {
+    head = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+    head = min(head, V);
+    vecs = (V - head) / kV;
+    edge = V - vecs * kV;
+  }
+  __device__ __forceinline__ int edge_column(int e) const { return e < head ? e : vecs * kV + e; }
+};
+
+// Running maximum and sums of exp((z - max) / tau) and, with kTwo, exp(z - max) over the values a thread has seen
+template <bool kTwo>
+struct Running {
+  float m = -INFINITY, st = 0.f, s1 = 0.f;
+  float c;  // log2(e) / tau
+  __device__ __forceinline__ explicit Running(float inv_tau) : c(inv_tau * 1.4426950409f) {}
+  __device__ __forceinline__ void raise(float to) {
+    if (to > m) {
+      st *= exp2_fast((m - to) * c);
+      if (kTwo) s1 *= exp2_fast((m - to) * 1.4426950409f);
+      m = to;
     }
-    const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
-    float m = -INFINITY, st = 0.f, s1 = 0.f;
-    for (int64_t c = threadIdx.x * kV; c < d.V; c += kRowThreads * kV) {
-      float f[kV];
-      load_vec<T, kV>(z + c, f);
-      float lm = f[0];
+  }
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }  // -inf - -inf would be NaN
+  template <int n>
+  __device__ __forceinline__ void add(const float* f) {
+    const float b = base();
+    if constexpr (n % 2 == 0) {
+      const F2 minus = f2(-b), cc = f2(c);
+      F2 t = f2(0.f), o = f2(0.f);
 #pragma unroll
-      for (int k = 1; k < kV; ++k) lm = fmaxf(lm, f[k]);
-      const float nm = fmaxf(m, lm);
-      if (nm == -INFINITY) {
-#pragma unroll
-        for (int k = 0; k < kV; ++k)
-          if (f[k] != f[k]) st = s1 = NAN;  // fmaxf drops NaN: the row has to show it
-        continue;
+      for (int i = 0; i < n; i += 2) {
+        const F2 x = add2(f2(f[i], f[i + 1]), minus);
+        const float2 y = split(mul2(x, cc));
+        t = add2(t, f2(exp2_fast(y.x), exp2_fast(y.y)));
+        if (kTwo) {
+          const float2 y1 = split(mul2(x, f2(1.4426950409f)));
+          o = add2(o, f2(exp2_fast(y1.x), exp2_fast(y1.y)));
+        }
       }
-      float at = 0.f, a1 = 0.f;
+      const float2 a = split(t), a1 = split(o);
+      st += a.x + a.y;
+      if (kTwo) s1 += a1.x + a1.y;
+    } else {
 #pragma unroll
-      for (int k = 0; k < kV; ++k) {
-        at += __expf((f[k] - nm) * inv_tau);
-        if (kHard) a1 += __expf(f[k] - nm);
+      for (int i = 0; i < n; ++i) {
+        st += exp2_fast((f[i] - b) * c);
+        if (kTwo) s1 += exp2_fast((f[i] - b) * 1.4426950409f);
       }
-      st = st * __expf((m - nm) * inv_tau) + at;
-      if (kHard) s1 = s1 * __expf(m - nm) + a1;
-      m = nm;
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  }
+};
+
+// d loss / d z from a value of z: exp((z - m) / tau) * iq + exp(z - m) * i1
+template <bool kTwo>
+struct Slope {
+  float m, c, iq, i1;
+  __device__ __forceinline__ float operator()(float z) const {
+    float o = exp2_fast((z - m) * c) * iq;
+    if (kTwo) o += exp2_fast((z - m) * 1.4426950409f) * i1;
+    return o;
+  }
+};
+
+constexpr int kAhead = 4;  // vectors of a thread that are on their way
+
+// A thread's vectors of a row, kAhead of them requested before the first is used: next() hands out the oldest and asks for
+// another in its place.
+template <typename T, int kThreads>
+struct Walk {
+  static constexpr int kV = Row<T>::kV;
+  Pack<T, kV> v[kAhead];
+  const T* at;  // the row's first vector
+  int vecs;
+  __device__ __forceinline__ void begin(const T* z, const Row<T>& row) {
+    at = z + row.head;
+    vecs = row.vecs;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, m, o), ot = __shfl_xor_sync(0xffffffffu, st, o);
-      const float o1 = kHard ? __shfl_xor_sync(0xffffffffu, s1, o) : 0.f;
-      join<kHard>(m, st, s1, om, ot, o1, inv_tau);
+    for (int u = 0; u < kAhead; ++u) ask(u, threadIdx.x + u * kThreads);
+  }
+  __device__ __forceinline__ void ask(int u, int i) {
+    if (i < vecs) v[u] = *reinterpret_cast<const Pack<T, kV>*>(at + i * (int64_t)kV);
+  }
+  // f(values, index) for every vector of this thread
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kThreads;
+        if (i < vecs) {
+          float x[kV];
+          unpack<T, kV>(v[u], x);
+          ask(u, i + kAhead * kThreads);
+          f(x, i);
+        }
+      }
     }
-    __syncthreads();
-    if (lane == 0) {
-      sm[0][warp] = m;
-      sm[1][warp] = st;
-      sm[2][warp] = s1;
+  }
+};
+
+// the gradient of one row but for the named places
+template <typename T, int kThreads, bool kTwo>
+__device__ __forceinline__ void row_gradient(const Row<T>& row, const T* z, T* g, Walk<T, kThreads>& walk, const Slope<kTwo>& slope) {
+  constexpr int kV = Row<T>::kV;
+  const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+  for (int e = threadIdx.x; e < row.edge; e += kThreads) {
+    const int c = row.edge_column(e);
+    g[c] = from_f32<T>(slope(to_f32(z[c])));
+  }
+  walk.each([&](float* f, int i) {
+#pragma unroll
+    for (int k = 0; k < kV; ++k) f[k] = slope(f[k]);
+    T* to = g + row.head + i * (int64_t)kV;
+    if (same) {
+      const Pack<T, kV> o = pack<T, kV>(f);
+      __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&o));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kV; ++k) to[k] = from_f32<T>(f[k]);
     }
-    __syncthreads();
-    m = -INFINITY, st = 0.f, s1 = 0.f;
-    for (int w = 0; w < kRowThreads / 32; ++w) join<kHard>(m, st, s1, sm[0][w], sm[1][w], sm[2][w], inv_tau);
-    // cross entropy of the teacher's entries against q
-    const float log_st = logf(st);
-    float ce = 0.f;
-    for (int k = threadIdx.x; k < d.K; k += kRowThreads) {
-      const float p = d.p[r * d.K + k];
-      if (p != 0.f) ce += p * ((to_f32(z[id_at(d, r * d.K + k)]) - m) * inv_tau - log_st);
+  });
+}
+template <typename T, int kThreads>
+__device__ __forceinline__ void row_zeros(T* g, int V) {
+  constexpr int kV = Row<T>::kV;
+  const Row<T> row(g, V);
+  for (int e = threadIdx.x; e < row.edge; e += kThreads) g[row.edge_column(e)] = from_f32<T>(0.f);
+  for (int i = threadIdx.x; i < row.vecs; i += kThreads) *reinterpret_cast<uint4*>(g + row.head + i * (int64_t)kV) = make_uint4(0, 0, 0, 0);
+}
+
+// The places that the teacher or the target names, each written once, by the warp of the first entry that names it: a warp per
+// entry, whose lanes look through the others. The rest of the row's gradient has been written and a barrier passed.
+template <typename T, int kThreads, bool kTwo>
+__device__ __forceinline__ void named_places(const mb_distill_t& d, int64_t r, const T* z, T* g, const Slope<kTwo>& slope, float a_soft,
+                                             float a_hard, const int* ids, const float* p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = a_hard != 0.f ? d.targets[r] : -1;
+  const bool staged = d.K <= kStaged;
+  for (int k = threadIdx.x >> 5; k <= d.K; k += kThreads / 32) {
+    const int64_t j = k == d.K ? t : staged ? (int64_t)ids[k] : id_at(d, r * d.K + k);
+    if (j < 0 || j >= d.V) continue;
+    bool earlier = false;
+    float sum = 0.f;
+    for (int i = lane; i < d.K; i += 32) {
+      if ((staged ? (int64_t)ids[i] : id_at(d, r * d.K + i)) == j) {
+        earlier |= i < k;
+        sum += staged ? p[i] : d.p[r * d.K + i];
+      }
     }
-    ce = block_reduce_sum<kRowThreads>(ce, red);
-    if (threadIdx.x == 0) {
-      d.stats[r * 3] = m;
-      d.stats[r * 3 + 1] = 1.f / st;
-      d.stats[r * 3 + 2] = kHard ? 1.f / s1 : 0.f;
-      float l = d.hard < 1.f ? (1.f - d.hard) * d.tau * d.tau * (d.entropy[r] - ce) : 0.f;
-      if (kHard) l += d.hard * (logf(s1) + m - to_f32(z[d.targets[r]]));
-      d.row_loss[r] = l;
-    }
+    if (__any_sync(0xffffffffu, earlier)) continue;
+    sum = warp_reduce_sum(sum);
+    if (lane == 0) g[j] = from_f32<T>(slope(to_f32(z[j])) - sum * a_soft - (j == t ? a_hard : 0.f));
   }
 }
 
-// loss = factor * sum of the row losses, in a fixed order (one CTA)
-__global__ void __launch_bounds__(1024) distill_sum_kernel(const mb_distill_t d) {
-  __shared__ float red[32];
-  float s = 0.f;
-  for (int64_t r = threadIdx.x; r < d.rows; r += 1024) s += d.row_loss[r];
-  s = block_reduce_sum<1024>(s, red);
-  if (threadIdx.x == 0) d.loss[0] = s * d.factor[0];
+// the row's teacher entries in shared memory, ids outside the vocabulary as -1
+template <int kThreads>
+__device__ __forceinline__ void stage_entries(const mb_distill_t& d, int64_t r, int* ids, float* p) {
+  if (d.K > kStaged) return;
+  for (int k = threadIdx.x; k < d.K; k += kThreads) {
+    const int64_t id = id_at(d, r * d.K + k);
+    ids[k] = id >= 0 && id < d.V ? (int)id : -1;
+    p[k] = d.p[r * d.K + k];
+  }
 }
 
-template <typename T, int kV, bool kHard>
-__global__ void __launch_bounds__(kRowThreads)
-    distill_grad_kernel(const mb_distill_t d, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
+// kTwo: the two terms need different exponentials (a hard term, and tau is not 1)
+template <typename T, int kThreads, bool kTwo>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
+    distill_row_kernel(const mb_distill_t d, T* __restrict__ grad, int64_t grad_stride) {
+  constexpr int kV = Row<T>::kV, kWarps = kThreads / 32;
+  __shared__ float red[4][kWarps];
+  __shared__ int ids[kStaged];
+  __shared__ float probs[kStaged];
+  __shared__ int shared_count;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float inv_tau = 1.f / d.tau;
-  const float sc = d.factor[0] * gout[0], a_soft = (1.f - d.hard) * d.tau * sc, a_hard = d.hard * sc;
+  const float factor = row_factor<kThreads>(d, &shared_count);
+  const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
   for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
     const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
     T* g = grad + r * grad_stride;
-    const bool live = d.live[r];
-    const float m = live ? d.stats[r * 3] : 0.f;
-    const float iq = live ? d.stats[r * 3 + 1] * a_soft : 0.f, i1 = live && kHard ? d.stats[r * 3 + 2] * a_hard : 0.f;
-    auto slope = [&](float v) {
-      float o = __expf((v - m) * inv_tau) * iq;
-      if (kHard) o += __expf(v - m) * i1;
-      return o;
-    };
-    for (int64_t c = threadIdx.x * kV; c < d.V; c += kRowThreads * kV) {
-      float f[kV];
-      if (live) load_vec<T, kV>(z + c, f);
+    if (!d.live[r]) {
+      if (threadIdx.x == 0) d.row_loss[r] = 0.f;
+      if (grad) row_zeros<T, kThreads>(g, d.V);
+      continue;
+    }
+    const Row<T> row(z, d.V);
+    Walk<T, kThreads> walk;
+    walk.begin(z, row);
+    __syncthreads();  // the row before is done with the staged entries
+    stage_entries<kThreads>(d, r, ids, probs);
+    // this thread's teacher entry, on its way while the row is read
+    float my_p = 0.f, my_z = 0.f;
+    if (threadIdx.x < d.K) {
+      my_p = d.p[r * d.K + threadIdx.x];
+      if (my_p != 0.f) my_z = to_f32(z[id_at(d, r * d.K + threadIdx.x)]);
+    }
+    Running<kTwo> run(inv_tau);
+    walk.each([&](float* f, int) {
+      float top = f[0];
 #pragma unroll
-      for (int k = 0; k < kV; ++k) f[k] = live ? slope(f[k]) : 0.f;
-      store_vec<T, kV>(g + c, f);
+      for (int k = 1; k < kV; ++k) top = fmaxf(top, f[k]);
+      run.raise(top);
+      run.template add<kV>(f);
+    });
+    for (int e = threadIdx.x; e < row.edge; e += kThreads) {
+      const float f = to_f32(z[row.edge_column(e)]);
+      run.raise(f);
+      run.template add<1>(&f);
     }
-    if (!live) continue;
+    if (grad) walk.begin(z, row);  // the second walk's first vectors
+    // (max, sums) of the warp, then of the CTA: one barrier
+    float m = warp_reduce_max(run.m);
+    float st = warp_reduce_sum(run.st * exp2_fast((run.m - m) * run.c));
+    float s1 = kTwo ? warp_reduce_sum(run.s1 * exp2_fast((run.m - m) * 1.4426950409f)) : 0.f;
+    // a warp that saw nothing but -inf has NaN here; it counts with nothing, unless it really saw NaN
+    if (m == -INFINITY && warp_reduce_sum(run.st) == 0.f) st = s1 = 0.f;
+    if (lane == 0) {
+      red[0][warp] = m;
+      red[1][warp] = st;
+      red[2][warp] = s1;
+    }
     __syncthreads();
-    // the places that the teacher or the target names, each written once by the first entry that names it
-    const int64_t t = kHard ? d.targets[r] : -1;
-    for (int k = threadIdx.x; k < d.K + (kHard ? 1 : 0); k += kRowThreads) {
-      const int64_t j = k < d.K ? id_at(d, r * d.K + k) : t;
-      if (j < 0 || j >= d.V) continue;
-      bool first = true;
-      float p = 0.f;
-      for (int i = 0; i < d.K && first; ++i) {
-        if (id_at(d, r * d.K + i) != j) continue;
-        if (i < k) first = false;
-        p += d.p[r * d.K + i];
-      }
-      if (first) g[j] = from_f32<T>(slope(to_f32(z[j])) - p * a_soft - (j == t ? a_hard : 0.f));
+    const float wm = red[0][lane % kWarps];
+    m = warp_reduce_max(wm);
+    const bool mine = lane < kWarps;
+    st = warp_reduce_sum(mine ? red[1][lane % kWarps] * exp2_fast((wm - m) * run.c) : 0.f);
+    s1 = kTwo ? warp_reduce_sum(mine ? red[2][lane % kWarps] * exp2_fast((wm - m) * 1.4426950409f) : 0.f) : st;
+    const Slope<kTwo> slope{m, run.c, kTwo ? a_soft / st : (a_soft + a_hard) / st, a_hard / s1};
+    // the teacher's entries against q, but for log(st)
+    float ce = my_p != 0.f ? my_p * (my_z - m) * inv_tau : 0.f;
+    for (int k = threadIdx.x + kThreads; k < d.K; k += kThreads) {
+      const float p = d.p[r * d.K + k];
+      if (p != 0.f) ce += p * (to_f32(z[id_at(d, r * d.K + k)]) - m) * inv_tau;
     }
+    ce = warp_reduce_sum(ce);
+    if (lane == 0) red[3][warp] = ce;
+    if (grad) row_gradient<T, kThreads, kTwo>(row, z, g, walk, slope);
+    __syncthreads();
+    if (grad) named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
+    if (warp == 0) {
+      ce = warp_reduce_sum(mine ? red[3][lane % kWarps] : 0.f);
+      if (lane == 0) {
+        d.stats[r * 3] = m;
+        d.stats[r * 3 + 1] = 1.f / st;
+        d.stats[r * 3 + 2] = 1.f / s1;
+        // the probabilities sum to 1, so log(st) stands outside the sum
+        float l = d.hard < 1.f ? (1.f - d.hard) * d.tau * d.tau * (d.entropy[r] - ce + logf(st)) : 0.f;
+        if (d.hard > 0.f) l += d.hard * (logf(s1) + m - to_f32(z[d.targets[r]]));
+        d.row_loss[r] = l;
+      }
+    }
+  }
+  // the last CTA to get here adds the row losses up, in a fixed order
+  __shared__ bool last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(d.counts + kTopCtas, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  float s = 0.f;
+  for (int64_t r = threadIdx.x; r < d.rows; r += kThreads) s += __ldcg(d.row_loss + r);
+  s = block_reduce_sum<kThreads>(s, red[0]);
+  if (threadIdx.x == 0) d.loss[0] = s * factor;
+}
+
+// the backward pass on its own: the logits once more
+template <typename T, int kThreads, bool kTwo>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
+    distill_grad_kernel(const mb_distill_t d, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
+  __shared__ int ids[kStaged];
+  __shared__ float probs[kStaged];
+  __shared__ int shared_count;
+  const float factor = row_factor<kThreads>(d, &shared_count) * gout[0];
+  const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
+  for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
+    const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
+    T* g = grad + r * grad_stride;
+    if (!d.live[r]) {
+      row_zeros<T, kThreads>(g, d.V);
+      continue;
+    }
+    const Row<T> row(z, d.V);
+    Walk<T, kThreads> walk;
+    walk.begin(z, row);
+    __syncthreads();  // the row before is done with the staged entries
+    stage_entries<kThreads>(d, r, ids, probs);
+    const float iq = d.stats[r * 3 + 1];
+    const Slope<kTwo> slope{d.stats[r * 3], 1.4426950409f / d.tau, kTwo ? a_soft * iq : (a_soft + a_hard) * iq, a_hard * d.stats[r * 3 + 2]};
+    row_gradient<T, kThreads, kTwo>(row, z, g, walk, slope);
+    __syncthreads();
+    named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
   }
 }
 
-inline unsigned row_grid(int64_t rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
+template <typename T>
+__global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_t n, const float* __restrict__ s) {
+  const float f = s[0];
+  if (f == 1.f) return;
+  constexpr int kV = 16 / sizeof(T);
+  const int64_t vecs = n / kV;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < vecs; i += gridDim.x * 256ll) {
+    float v[kV];
+    load_vec<T, kV>(x + i * kV, v);
+#pragma unroll
+    for (int k = 0; k < kV; ++k) v[k] *= f;
+    store_vec<T, kV>(x + i * kV, v);
+  }
+  for (int64_t i = vecs * kV + blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) x[i] = from_f32<T>(to_f32(x[i]) * f);
+}
+
+// One CTA per row at a time. Long rows get LONG threads and 1024 / LONG CTAs per SM, so that the rows in work fit L2 between
+// their two walks; up to 8192 words 128 threads hold a row's latency and many CTAs share an SM.
+constexpr int kLongRow = 8192, kLongThreads = 512;
+inline unsigned row_ctas(int64_t rows, int V) {
+  const int64_t most = V > kLongRow ? kSms * (1024 / kLongThreads) : kSms * 8;
+  return (unsigned)(rows < most ? rows : most);
+}
 
 template <typename T>
-int fwd(const mb_distill_t& d, cudaStream_t s) {
-  constexpr int kV = 16 / sizeof(T);
-  const bool vec = d.V % kV == 0 && d.stride % kV == 0 && is_aligned(d.logits, 16);
-  auto k = d.hard > 0.f ? (vec ? distill_row_kernel<T, kV, true> : distill_row_kernel<T, 1, true>)
-                        : (vec ? distill_row_kernel<T, kV, false> : distill_row_kernel<T, 1, false>);
-  k<<<row_grid(d.rows), kRowThreads, 0, s>>>(d);
+int fwd(const mb_distill_t& d, void* grad, int64_t grad_stride, cudaStream_t s) {
+  const bool two = d.hard > 0.f && d.tau != 1.f;
+  if (d.V > kLongRow) {
+    auto k = two ? distill_row_kernel<T, kLongThreads, true> : distill_row_kernel<T, kLongThreads, false>;
+    k<<<row_ctas(d.rows, d.V), kLongThreads, 0, s>>>(d, (T*)grad, grad_stride);
+  } else {
+    auto k = two ? distill_row_kernel<T, 128, true> : distill_row_kernel<T, 128, false>;
+    k<<<row_ctas(d.rows, d.V), 128, 0, s>>>(d, (T*)grad, grad_stride);
+  }
   return check_launch();
 }
 
 template <typename T>
 int bwd(const mb_distill_t& d, const float* gout, void* grad, int64_t grad_stride, cudaStream_t s) {
-  constexpr int kV = 16 / sizeof(T);
-  const bool vec = d.V % kV == 0 && d.stride % kV == 0 && grad_stride % kV == 0 && is_aligned(d.logits, 16) && is_aligned(grad, 16);
-  auto k = d.hard > 0.f ? (vec ? distill_grad_kernel<T, kV, true> : distill_grad_kernel<T, 1, true>)
-                        : (vec ? distill_grad_kernel<T, kV, false> : distill_grad_kernel<T, 1, false>);
-  k<<<row_grid(d.rows), kRowThreads, 0, s>>>(d, gout, (T*)grad, grad_stride);
+  const bool two = d.hard > 0.f && d.tau != 1.f;
+  if (d.V > kLongRow) {
+    auto k = two ? distill_grad_kernel<T, kLongThreads, true> : distill_grad_kernel<T, kLongThreads, false>;
+    k<<<row_ctas(d.rows, d.V), kLongThreads, 0, s>>>(d, gout, (T*)grad, grad_stride);
+  } else {
+    auto k = two ? distill_grad_kernel<T, 128, true> : distill_grad_kernel<T, 128, false>;
+    k<<<row_ctas(d.rows, d.V), 128, 0, s>>>(d, gout, (T*)grad, grad_stride);
+  }
   return check_launch();
 }
 
 bool sane(const mb_distill_t& d) {
-  return d.V > 0 && d.K > 0 && d.tau > 0.f && d.hard >= 0.f && d.hard <= 1.f && (d.hard == 0.f || d.targets || d.rows <= 0) &&
+  return d.rows > 0 && d.V > 0 && d.K > 0 && d.tau > 0.f && d.hard >= 0.f && d.hard <= 1.f && (d.hard == 0.f || d.targets) &&
          (d.top_dtype == MB_F32 || d.top_dtype == MB_BF16 || d.top_dtype == MB_F16);
 }
 
 }  // namespace
 
-extern "C" int mb_distill_fwd(const mb_distill_t* d, void* stream) {
+extern "C" int mb_distill_fwd(const mb_distill_t* d, void* grad, int64_t grad_stride, void* stream) {
   if (!sane(*d)) return MB_ERR_ARG;
   cudaStream_t s = MB_STREAM(stream);
-  if (d->rows > 0) {
-    distill_teacher_kernel<<<row_grid(d->rows), kTopThreads, 0, s>>>(*d);
-    if (check_launch()) return MB_ERR_LAUNCH;
-  }
-  distill_factor_kernel<<<1, 1024, 0, s>>>(*d);
+  distill_teacher_kernel<<<top_ctas(d->rows), kTopThreads, 0, s>>>(*d);
   if (check_launch()) return MB_ERR_LAUNCH;
-  if (d->rows > 0) {
-    int rc = MB_ERR_ARG;
-    if (d->dtype == MB_BF16) rc = fwd<__nv_bfloat16>(*d, s);
-    if (d->dtype == MB_F16) rc = fwd<__half>(*d, s);
-    if (d->dtype == MB_F32) rc = fwd<float>(*d, s);
-    if (rc) return rc;
+  switch (d->dtype) {
+    case MB_BF16: return fwd<__nv_bfloat16>(*d, grad, grad_stride, s);
+    case MB_F16: return fwd<__half>(*d, grad, grad_stride, s);
+    case MB_F32: return fwd<float>(*d, grad, grad_stride, s);
+    default: return MB_ERR_ARG;
   }
-  distill_sum_kernel<<<1, 1024, 0, s>>>(*d);
-  return check_launch();
 }
 
 extern "C" int mb_distill_bwd(const mb_distill_t* d, const float* gout, void* grad, int64_t grad_stride, void* stream) {
   if (!sane(*d)) return MB_ERR_ARG;
-  if (d->rows <= 0) return MB_OK;
   switch (d->dtype) {
     case MB_BF16: return bwd<__nv_bfloat16>(*d, gout, grad, grad_stride, MB_STREAM(stream));
     case MB_F16: return bwd<__half>(*d, gout, grad, grad_stride, MB_STREAM(stream));
     case MB_F32: return bwd<float>(*d, gout, grad, grad_stride, MB_STREAM(stream));
     default: return MB_ERR_ARG;
   }
+}
+
+extern "C" int mb_scale_by(void* x, int64_t n, int dtype, const float* s, void* stream) {
+  if (n <= 0) return MB_OK;
+  if (!is_aligned(x, 16)) return MB_ERR_ALIGN;
+  int64_t grid = (n / 8 + 255) / 256;
+  grid = grid < 1 ? 1 : grid > kSms * 8 ? kSms * 8 : grid;
+  switch (dtype) {
+    case MB_BF16: scale_by_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((__nv_bfloat16*)x, n, s); break;
+    case MB_F16: scale_by_kernel<__half><<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((__half*)x, n, s); break;
+    case MB_F32: scale_by_kernel<float><<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((float*)x, n, s); break;
+    default: return MB_ERR_ARG;
+  }
+  return check_launch();
 }

@@ -252,17 +252,21 @@ typedef struct {
   int64_t ignore_index;
   float tau, hard, scale;
   int mean;        // 1: over the rows that take part, 0: sum
-  float* p;        // scratch [rows, K]: the teacher's probabilities
-  float* entropy;  // scratch [rows]: sum_k p_k log p_k
-  int* live;       // scratch [rows]
-  float* factor;   // [1]: scale, or scale / number of rows that take part
-  float* stats;    // [rows, 3]: max, 1 / sum exp((z - max) / tau), 1 / sum exp(z - max)
-  float* row_loss; // scratch [rows]
-  float* loss;     // [1]
+  float* p;         // scratch [rows, K]: the teacher's probabilities
+  float* entropy;   // scratch [rows]: sum_k p_k log p_k
+  int* live;        // scratch [rows]
+  float* stats;     // [rows, 3]: max, 1 / sum exp((z - max) / tau), 1 / sum exp(z - max)
+  float* row_loss;  // scratch [rows]
+  int* counts;      // scratch [MB_DISTILL_COUNTS]
+  float* loss;      // [1]
 } mb_distill_t;
-int mb_distill_fwd(const mb_distill_t* d, void* stream);
-// grad[rows, V] = d loss / d logits * gout[0], from the p, live, factor and stats that the forward call left
+#define MB_DISTILL_COUNTS 1200
+// The loss and, where grad is not null, grad[rows, V] = d loss / d logits: the logits are read from memory once for both.
+int mb_distill_fwd(const mb_distill_t* d, void* grad, int64_t grad_stride, void* stream);
+// grad[rows, V] = d loss / d logits * gout[0], from the scratch and stats that a forward call without grad left.
 int mb_distill_bwd(const mb_distill_t* d, const float* gout, void* grad, int64_t grad_stride, void* stream);
+// x[0 .. n) *= s[0], in place; leaves x alone when s[0] is 1 (x: dtype, 16-byte aligned)
+int mb_scale_by(void* x, int64_t n, int dtype, const float* s, void* stream);
 // Gated projection (gated_gemm.cu): h[T, F] = act(x Wg^T) * (x Wu^T) for bf16 x[T, K] and w[2F, K] (gate rows first); gu
 // (may be null) receives the two projections [T, 2F]. act: 0 SiLU, 1 GELU, 2 GELU with tanh. F, K and the pitches are
 // multiples of 8, all addresses 16-byte aligned. The backward call turns dh and gu into dgu[T, 2F], the gradient of x w^T.
