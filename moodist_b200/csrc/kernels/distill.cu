@@ -173,10 +173,45 @@ struct Running {
   }
 };
 
+// the largest of a vector's values, NaN left out
+template <typename T, int N>
+__device__ __forceinline__ float largest(const Pack<T, N>& p, const float* f) {
+  if constexpr (sizeof(T) == 2) {
+    using P = typename PairOf<T>::type;
+    P top = *reinterpret_cast<const P*>(&p.w[0]);
+#pragma unroll
+    for (int i = 1; i < N / 2; ++i) top = __hmax2(top, *reinterpret_cast<const P*>(&p.w[i]));
+    const float2 t = pair_to_f32<T>(*reinterpret_cast<const uint32_t*>(&top));
+    return fmaxf(t.x, t.y);
+  } else {
+    float top = f[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) top = fmaxf(top, f[k]);
+    return top;
+  }
+}
+
 // d loss / d z from a value of z: exp((z - m) / tau) * iq + exp(z - m) * i1
 template <bool kTwo>
 struct Slope {
   float m, c, iq, i1;
+  template <int n>
+  __device__ __forceinline__ void all(float* f) const {
+    const F2 minus = f2(-m), cc = f2(c), q = f2(iq), one = f2(1.4426950409f), q1 = f2(i1);
+#pragma unroll
+    for (int k = 0; k < n; k += 2) {
+      const F2 x = add2(f2(f[k], f[k + 1]), minus);
+      const float2 y = split(mul2(x, cc));
+      F2 o = mul2(f2(exp2_fast(y.x), exp2_fast(y.y)), q);
+      if (kTwo) {
+        const float2 y1 = split(mul2(x, one));
+        o = fma2(f2(exp2_fast(y1.x), exp2_fast(y1.y)), q1, o);
+      }
+      const float2 r = split(o);
+      f[k] = r.x;
+      f[k + 1] = r.y;
+    }
+  }
   __device__ __forceinline__ float operator()(float z) const {
     float o = exp2_fast((z - m) * c) * iq;
     if (kTwo) o += exp2_fast((z - m) * 1.4426950409f) * i1;
@@ -184,55 +219,94 @@ struct Slope {
   }
 };
 
-constexpr int kAhead = 4;  // vectors of a thread that are on their way
-
-// A thread's vectors of a row, kAhead of them requested before the first is used: next() hands out the oldest and asks for
-// another in its place.
-template <typename T, int kThreads>
-struct Walk {
+// The vectors that a thread is going to read, in order: those of its rows, each row once or, with the gradient, twice. They travel
+// kDepth ahead into the thread's own slots of shared memory, over the ends of walks and rows, so that neither the latency of
+// memory nor the barriers between the walks leave the memory idle (four vectors ahead in registers, begun anew for each
+// walk: 643 us at 4096 x 128256).
+template <typename T, int kThreads, int kDepth>
+struct Stream {
   static constexpr int kV = Row<T>::kV;
-  Pack<T, kV> v[kAhead];
-  const T* at;  // the row's first vector
-  int vecs;
-  __device__ __forceinline__ void begin(const T* z, const Row<T>& row) {
-    at = z + row.head;
-    vecs = row.vecs;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) ask(u, threadIdx.x + u * kThreads);
+  static constexpr int kBytes = kDepth * kThreads * 16;
+  uint8_t* slots;
+  const mb_distill_t* d;
+  const T* at;   // the next vector to ask for
+  int64_t row;   // its row
+  int left;      // how many of this walk are still to be asked for
+  int walks;     // walks over the row after this one
+  int per_row;   // walks per row, less one
+  int slot;
+
+  __device__ __forceinline__ static int mine(int vecs) { return vecs > (int)threadIdx.x ? (vecs - (int)threadIdx.x + kThreads - 1) / kThreads : 0; }
+  __device__ __forceinline__ void start_walk() {
+    const T* z = reinterpret_cast<const T*>(d->logits) + row * d->stride;
+    const Row<T> shape(z, d->V);
+    at = z + shape.head + threadIdx.x * (int64_t)kV;
+    left = mine(shape.vecs);
   }
-  __device__ __forceinline__ void ask(int u, int i) {
-    if (i < vecs) v[u] = *reinterpret_cast<const Pack<T, kV>*>(at + i * (int64_t)kV);
+  __device__ __forceinline__ void seek() {
+    while (row < d->rows && !d->live[row]) row += gridDim.x;
+    if (row < d->rows) {
+      walks = per_row;
+      start_walk();
+    }
   }
-  // f(values, index) for every vector of this thread
-  template <typename F>
-  __device__ __forceinline__ void each(F f) {
-    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kAhead) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int i = i0 + u * kThreads;
-        if (i < vecs) {
-          float x[kV];
-          unpack<T, kV>(v[u], x);
-          ask(u, i + kAhead * kThreads);
-          f(x, i);
-        }
+  __device__ __forceinline__ void begin(uint8_t* smem, const mb_distill_t& args, int64_t first, bool twice) {
+    slots = smem + threadIdx.x * 16;
+    d = &args;
+    row = first;
+    left = 0;
+    per_row = twice;
+    slot = 0;
+    seek();
+#pragma unroll 1
+    for (int i = 0; i < kDepth; ++i) ask(i);
+  }
+  __device__ __forceinline__ void ask(int into) {
+    while (left == 0 && row < d->rows) {
+      if (walks > 0) {
+        --walks;
+        start_walk();
+        if (left == 0) walks = 0;  // a row without vectors for this thread
+      } else {
+        row += gridDim.x;
+        seek();
       }
+    }
+    if (left > 0) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slots + into * kThreads * 16)), "l"(at)
+                   : "memory");
+      at += kThreads * kV;
+      --left;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // f(vector, its index in the row) for this thread's vectors of one walk
+  template <typename F>
+  __device__ __forceinline__ void each(int vecs, F f) {
+    for (int i = threadIdx.x; i < vecs; i += kThreads) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      const Pack<T, kV> v = *reinterpret_cast<const Pack<T, kV>*>(slots + slot * kThreads * 16);
+      float x[kV];
+      unpack<T, kV>(v, x);
+      f(v, x, i);
+      // the vector's values have been used, so its slot is free
+      ask(slot);
+      if (++slot == kDepth) slot = 0;
     }
   }
 };
 
 // the gradient of one row but for the named places
-template <typename T, int kThreads, bool kTwo>
-__device__ __forceinline__ void row_gradient(const Row<T>& row, const T* z, T* g, Walk<T, kThreads>& walk, const Slope<kTwo>& slope) {
+template <typename T, int kThreads, bool kTwo, typename S>
+__device__ __forceinline__ void row_gradient(const Row<T>& row, const T* z, T* g, S& stream, const Slope<kTwo>& slope) {
   constexpr int kV = Row<T>::kV;
   const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   for (int e = threadIdx.x; e < row.edge; e += kThreads) {
     const int c = row.edge_column(e);
     g[c] = from_f32<T>(slope(to_f32(z[c])));
   }
-  walk.each([&](float* f, int i) {
-#pragma unroll
-    for (int k = 0; k < kV; ++k) f[k] = slope(f[k]);
+  stream.each(row.vecs, [&](const Pack<T, kV>&, float* f, int i) {
+    slope.template all<kV>(f);
     T* to = g + row.head + i * (int64_t)kV;
     if (same) {
       const Pack<T, kV> o = pack<T, kV>(f);
@@ -287,11 +361,15 @@ __device__ __forceinline__ void stage_entries(const mb_distill_t& d, int64_t r, 
   }
 }
 
+// vectors ahead: 80 KB per CTA of 512 threads, two CTAs per SM; 8 KB per CTA of 128, up to eight
+constexpr int depth_for(int threads) { return threads > 128 ? 10 : 4; }
+
 // kTwo: the two terms need different exponentials (a hard term, and tau is not 1)
 template <typename T, int kThreads, bool kTwo>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
-    distill_row_kernel(const mb_distill_t d, T* __restrict__ grad, int64_t grad_stride) {
+    distill_row_kernel(const __grid_constant__ mb_distill_t d, T* __restrict__ grad, int64_t grad_stride) {
   constexpr int kV = Row<T>::kV, kWarps = kThreads / 32;
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[4][kWarps];
   __shared__ int ids[kStaged];
   __shared__ float probs[kStaged];
@@ -300,6 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   const float inv_tau = 1.f / d.tau;
   const float factor = row_factor<kThreads>(d, &shared_count);
   const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
+  Stream<T, kThreads, depth_for(kThreads)> stream;
+  stream.begin(ring, d, blockIdx.x, grad != nullptr);
   for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
     const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
     T* g = grad + r * grad_stride;
@@ -309,8 +389,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       continue;
     }
     const Row<T> row(z, d.V);
-    Walk<T, kThreads> walk;
-    walk.begin(z, row);
     __syncthreads();  // the row before is done with the staged entries
     stage_entries<kThreads>(d, r, ids, probs);
     // this thread's teacher entry, on its way while the row is read
@@ -320,11 +398,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       if (my_p != 0.f) my_z = to_f32(z[id_at(d, r * d.K + threadIdx.x)]);
     }
     Running<kTwo> run(inv_tau);
-    walk.each([&](float* f, int) {
-      float top = f[0];
-#pragma unroll
-      for (int k = 1; k < kV; ++k) top = fmaxf(top, f[k]);
-      run.raise(top);
+    stream.each(row.vecs, [&](const Pack<T, kV>& v, const float* f, int) {
+      run.raise(largest(v, f));
       run.template add<kV>(f);
     });
     for (int e = threadIdx.x; e < row.edge; e += kThreads) {
@@ -332,7 +407,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       run.raise(f);
       run.template add<1>(&f);
     }
-    if (grad) walk.begin(z, row);  // the second walk's first vectors
     // (max, sums) of the warp, then of the CTA: one barrier
     float m = warp_reduce_max(run.m);
     float st = warp_reduce_sum(run.st * exp2_fast((run.m - m) * run.c));
@@ -359,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     }
     ce = warp_reduce_sum(ce);
     if (lane == 0) red[3][warp] = ce;
-    if (grad) row_gradient<T, kThreads, kTwo>(row, z, g, walk, slope);
+    if (grad) row_gradient<T, kThreads, kTwo>(row, z, g, stream, slope);
     __syncthreads();
     if (grad) named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
     if (warp == 0) {
@@ -392,12 +466,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 // the backward pass on its own: the logits once more
 template <typename T, int kThreads, bool kTwo>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
-    distill_grad_kernel(const mb_distill_t d, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
+    distill_grad_kernel(const __grid_constant__ mb_distill_t d, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ int ids[kStaged];
   __shared__ float probs[kStaged];
   __shared__ int shared_count;
   const float factor = row_factor<kThreads>(d, &shared_count) * gout[0];
   const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
+  Stream<T, kThreads, depth_for(kThreads)> stream;
+  stream.begin(ring, d, blockIdx.x, false);
   for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
     const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
     T* g = grad + r * grad_stride;
@@ -406,13 +483,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       continue;
     }
     const Row<T> row(z, d.V);
-    Walk<T, kThreads> walk;
-    walk.begin(z, row);
     __syncthreads();  // the row before is done with the staged entries
     stage_entries<kThreads>(d, r, ids, probs);
     const float iq = d.stats[r * 3 + 1];
     const Slope<kTwo> slope{d.stats[r * 3], 1.4426950409f / d.tau, kTwo ? a_soft * iq : (a_soft + a_hard) * iq, a_hard * d.stats[r * 3 + 2]};
-    row_gradient<T, kThreads, kTwo>(row, z, g, walk, slope);
+    row_gradient<T, kThreads, kTwo>(row, z, g, stream, slope);
     __syncthreads();
     named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
   }
@@ -442,30 +517,39 @@ inline unsigned row_ctas(int64_t rows, int V) {
   return (unsigned)(rows < most ? rows : most);
 }
 
-template <typename T>
-int fwd(const mb_distill_t& d, void* grad, int64_t grad_stride, cudaStream_t s) {
-  const bool two = d.hard > 0.f && d.tau != 1.f;
-  if (d.V > kLongRow) {
-    auto k = two ? distill_row_kernel<T, kLongThreads, true> : distill_row_kernel<T, kLongThreads, false>;
-    k<<<row_ctas(d.rows, d.V), kLongThreads, 0, s>>>(d, (T*)grad, grad_stride);
-  } else {
-    auto k = two ? distill_row_kernel<T, 128, true> : distill_row_kernel<T, 128, false>;
-    k<<<row_ctas(d.rows, d.V), 128, 0, s>>>(d, (T*)grad, grad_stride);
+template <auto kKernel, int kThreads, typename... Args>
+int launch(const mb_distill_t& d, cudaStream_t s, Args... args) {
+  constexpr int smem = depth_for(kThreads) * kThreads * 16;
+  static bool done[64];  // per kernel and device
+  if (smem > 48 * 1024) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return MB_ERR_DRIVER;
+    if (!done[device] && cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return MB_ERR_LAUNCH;
+    done[device] = true;
   }
+  kKernel<<<row_ctas(d.rows, d.V), kThreads, smem, s>>>(d, args...);
   return check_launch();
 }
 
+template <typename T, int kThreads, bool kTwo>
+int fwd_with(const mb_distill_t& d, void* grad, int64_t grad_stride, cudaStream_t s) {
+  return launch<distill_row_kernel<T, kThreads, kTwo>, kThreads>(d, s, (T*)grad, grad_stride);
+}
+template <typename T, int kThreads, bool kTwo>
+int bwd_with(const mb_distill_t& d, const float* gout, void* grad, int64_t grad_stride, cudaStream_t s) {
+  return launch<distill_grad_kernel<T, kThreads, kTwo>, kThreads>(d, s, gout, (T*)grad, grad_stride);
+}
+template <typename T>
+int fwd(const mb_distill_t& d, void* grad, int64_t grad_stride, cudaStream_t s) {
+  const bool two = d.hard > 0.f && d.tau != 1.f;
+  if (d.V > kLongRow) return two ? fwd_with<T, kLongThreads, true>(d, grad, grad_stride, s) : fwd_with<T, kLongThreads, false>(d, grad, grad_stride, s);
+  return two ? fwd_with<T, 128, true>(d, grad, grad_stride, s) : fwd_with<T, 128, false>(d, grad, grad_stride, s);
+}
 template <typename T>
 int bwd(const mb_distill_t& d, const float* gout, void* grad, int64_t grad_stride, cudaStream_t s) {
   const bool two = d.hard > 0.f && d.tau != 1.f;
-  if (d.V > kLongRow) {
-    auto k = two ? distill_grad_kernel<T, kLongThreads, true> : distill_grad_kernel<T, kLongThreads, false>;
-    k<<<row_ctas(d.rows, d.V), kLongThreads, 0, s>>>(d, gout, (T*)grad, grad_stride);
-  } else {
-    auto k = two ? distill_grad_kernel<T, 128, true> : distill_grad_kernel<T, 128, false>;
-    k<<<row_ctas(d.rows, d.V), 128, 0, s>>>(d, gout, (T*)grad, grad_stride);
-  }
-  return check_launch();
+  if (d.V > kLongRow) return two ? bwd_with<T, kLongThreads, true>(d, gout, grad, grad_stride, s) : bwd_with<T, kLongThreads, false>(d, gout, grad, grad_stride, s);
+  return two ? bwd_with<T, 128, true>(d, gout, grad, grad_stride, s) : bwd_with<T, 128, false>(d, gout, grad, grad_stride, s);
 }
 
 bool sane(const mb_distill_t& d) {

@@ -64,6 +64,17 @@ __device__ __forceinline__ uint32_t pair_from_f32<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+template <typename T>
+struct PairOf;
+template <>
+struct PairOf<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+template <>
+struct PairOf<__half> {
+  using type = __half2;
+};
+
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Pack<T, N>& p, float* f) {
   if constexpr (sizeof(T) == 4) {
