@@ -44,57 +44,66 @@ __device__ __forceinline__ bool entry(const mb_distill_t& d, int64_t i, float* t
   return *t != -INFINITY;
 }
 
-// One CTA per row: the teacher's probabilities over the valid entries (0 in the others), sum p log p, whether the row counts;
+// One warp per row: the teacher's probabilities over the valid entries (0 in the others), sum p log p, whether the row counts;
 // per CTA how many rows do. Readies the ticket of the row kernel.
-__global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const mb_distill_t d) {
-  __shared__ float red[kTopThreads / 32];
+__global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const __grid_constant__ mb_distill_t d) {
+  __shared__ int counts[kTopThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float inv_tau = 1.f / d.tau;
   int count = 0;
-  for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
+  for (int64_t r = blockIdx.x * (int64_t)(kTopThreads / 32) + warp; r < d.rows; r += (int64_t)gridDim.x * (kTopThreads / 32)) {
     const int64_t base = r * d.K;
     bool counts = true;
     if (d.targets) {
       const int64_t t = d.targets[r];
       counts = t != d.ignore_index && t >= 0 && t < d.V;
     }
-    float m = -INFINITY, any = 0.f;
-    float t;
-    for (int k = threadIdx.x; k < d.K; k += kTopThreads) {
+    float m = -INFINITY, t;
+    bool any = false;
+    for (int k = lane; k < d.K; k += 32) {
       if (entry(d, base + k, &t)) {
-        any = 1.f;
+        any = true;
         m = fmaxf(m, t);
       }
     }
-    m = block_reduce_max<kTopThreads>(m, red);
-    any = block_reduce_max<kTopThreads>(any, red);
-    const bool live = counts && any > 0.f;
+    m = warp_reduce_max(m);
+    const bool live = counts && __any_sync(0xffffffffu, any);
     float s = 0.f, e = 0.f;
-    for (int k = threadIdx.x; k < d.K; k += kTopThreads) {
+    for (int k = lane; k < d.K; k += 32) {
+      float w = 0.f;
       if (live && entry(d, base + k, &t)) {
         t = (t - m) * inv_tau;
-        const float w = expf(t);
+        w = expf(t);
         s += w;
         if (!(w <= 0.f)) e += w * t;  // weight 0: t may have overflowed to -inf; NaN goes on
       }
+      d.p[base + k] = w;
     }
-    s = block_reduce_sum<kTopThreads>(s, red);
-    e = block_reduce_sum<kTopThreads>(e, red);
-    const float inv = live ? 1.f / s : 0.f;
-    for (int k = threadIdx.x; k < d.K; k += kTopThreads)
-      d.p[base + k] = live && entry(d, base + k, &t) ? expf((t - m) * inv_tau) * inv : 0.f;
+    s = warp_reduce_sum(s);
+    e = warp_reduce_sum(e);
+    if (live) {
+      const float inv = 1.f / s;
+      for (int k = lane; k < d.K; k += 32) d.p[base + k] *= inv;
+    }
     count += live;
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
       d.live[r] = live;
-      d.entropy[r] = live ? e * inv - logf(s) : 0.f;
+      d.entropy[r] = live ? e / s - logf(s) : 0.f;
     }
   }
+  if (lane == 0) counts[warp] = count;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    for (int w = 1; w < kTopThreads / 32; ++w) count += counts[w];
     d.counts[blockIdx.x] = count;
     if (blockIdx.x == 0) d.counts[kTopCtas] = 0;
   }
 }
 
-inline __host__ __device__ int top_ctas(int64_t rows) { return (int)(rows < kTopCtas ? rows : kTopCtas); }
+inline __host__ __device__ int top_ctas(int64_t rows) {
+  const int64_t n = (rows + kTopThreads / 32 - 1) / (kTopThreads / 32);
+  return (int)(n < kTopCtas ? n : kTopCtas);
+}
 
 // scale, or scale over the number of rows that count; all threads of the CTA get it
 template <int kThreads>
@@ -130,63 +139,58 @@ struct Row {
   __device__ __forceinline__ int edge_column(int e) const { return e < head ? e : vecs * kV + e; }
 };
 
-// Running maximum and sums of exp((z - max) / tau) and, with kTwo, exp(z - max) over the values a thread has seen
+// Running maximum and sums of exp((z - max) / tau) and, with kTwo, exp(z - max) over the values a thread has seen; the sums as
+// pairs, which are added up at the end
+constexpr float kLog2e = 1.4426950409f;
 template <bool kTwo>
 struct Running {
-  float m = -INFINITY, st = 0.f, s1 = 0.f;
+  float m = -INFINITY;
+  F2 st = f2(0.f), s1 = f2(0.f);
   float c;  // log2(e) / tau
-  __device__ __forceinline__ explicit Running(float inv_tau) : c(inv_tau * 1.4426950409f) {}
+  __device__ __forceinline__ explicit Running(float inv_tau) : c(inv_tau * kLog2e) {}
   __device__ __forceinline__ void raise(float to) {
     if (to > m) {
-      st *= exp2_fast((m - to) * c);
-      if (kTwo) s1 *= exp2_fast((m - to) * 1.4426950409f);
+      st = mul2(st, f2(exp2_fast((m - to) * c)));
+      if (kTwo) s1 = mul2(s1, f2(exp2_fast((m - to) * kLog2e)));
       m = to;
     }
   }
   __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }  // -inf - -inf would be NaN
   template <int n>
   __device__ __forceinline__ void add(const float* f) {
-    const float b = base();
-    if constexpr (n % 2 == 0) {
-      const F2 minus = f2(-b), cc = f2(c);
-      F2 t = f2(0.f), o = f2(0.f);
+    const F2 minus = f2(-base()), cc = f2(c);
 #pragma unroll
-      for (int i = 0; i < n; i += 2) {
-        const F2 x = add2(f2(f[i], f[i + 1]), minus);
-        const float2 y = split(mul2(x, cc));
-        t = add2(t, f2(exp2_fast(y.x), exp2_fast(y.y)));
-        if (kTwo) {
-          const float2 y1 = split(mul2(x, f2(1.4426950409f)));
-          o = add2(o, f2(exp2_fast(y1.x), exp2_fast(y1.y)));
-        }
-      }
-      const float2 a = split(t), a1 = split(o);
-      st += a.x + a.y;
-      if (kTwo) s1 += a1.x + a1.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < n; ++i) {
-        st += exp2_fast((f[i] - b) * c);
-        if (kTwo) s1 += exp2_fast((f[i] - b) * 1.4426950409f);
+    for (int i = 0; i < n; i += 2) {
+      const F2 x = add2(f2(f[i], f[i + 1]), minus);
+      const float2 y = split(mul2(x, cc));
+      st = add2(st, f2(exp2_fast(y.x), exp2_fast(y.y)));
+      if (kTwo) {
+        const float2 y1 = split(mul2(x, f2(kLog2e)));
+        s1 = add2(s1, f2(exp2_fast(y1.x), exp2_fast(y1.y)));
       }
     }
   }
+  __device__ __forceinline__ void add_one(float z) {
+    raise(z);
+    st = add2(st, f2(exp2_fast((z - base()) * c), 0.f));
+    if (kTwo) s1 = add2(s1, f2(exp2_fast((z - base()) * kLog2e), 0.f));
+  }
 };
 
-// the largest of a vector's values, NaN left out
-template <typename T, int N>
-__device__ __forceinline__ float largest(const Pack<T, N>& p, const float* f) {
+// the largest value of n vectors, NaN left out
+template <typename T, int N, int n>
+__device__ __forceinline__ float largest(const Pack<T, N> (&p)[n]) {
   if constexpr (sizeof(T) == 2) {
     using P = typename PairOf<T>::type;
-    P top = *reinterpret_cast<const P*>(&p.w[0]);
+    P top = *reinterpret_cast<const P*>(&p[0].w[0]);
 #pragma unroll
-    for (int i = 1; i < N / 2; ++i) top = __hmax2(top, *reinterpret_cast<const P*>(&p.w[i]));
+    for (int i = 1; i < n * N / 2; ++i) top = __hmax2(top, *reinterpret_cast<const P*>(&p[i / (N / 2)].w[i % (N / 2)]));
     const float2 t = pair_to_f32<T>(*reinterpret_cast<const uint32_t*>(&top));
     return fmaxf(t.x, t.y);
   } else {
-    float top = f[0];
+    float top = __uint_as_float(p[0].w[0]);
 #pragma unroll
-    for (int k = 1; k < N; ++k) top = fmaxf(top, f[k]);
+    for (int i = 1; i < n * N; ++i) top = fmaxf(top, __uint_as_float(p[i / N].w[i % N]));
     return top;
   }
 }
@@ -197,7 +201,7 @@ struct Slope {
   float m, c, iq, i1;
   template <int n>
   __device__ __forceinline__ void all(float* f) const {
-    const F2 minus = f2(-m), cc = f2(c), q = f2(iq), one = f2(1.4426950409f), q1 = f2(i1);
+    const F2 minus = f2(-m), cc = f2(c), q = f2(iq), one = f2(kLog2e), q1 = f2(i1);
 #pragma unroll
     for (int k = 0; k < n; k += 2) {
       const F2 x = add2(f2(f[k], f[k + 1]), minus);
@@ -214,84 +218,99 @@ struct Slope {
   }
   __device__ __forceinline__ float operator()(float z) const {
     float o = exp2_fast((z - m) * c) * iq;
-    if (kTwo) o += exp2_fast((z - m) * 1.4426950409f) * i1;
+    if (kTwo) o += exp2_fast((z - m) * kLog2e) * i1;
     return o;
   }
 };
 
 // The vectors that a thread is going to read, in order: those of its rows, each row once or, with the gradient, twice. They travel
-// kDepth ahead into the thread's own slots of shared memory, over the ends of walks and rows, so that neither the latency of
-// memory nor the barriers between the walks leave the memory idle (four vectors ahead in registers, begun anew for each
-// walk: 643 us at 4096 x 128256).
+// kDepth steps of four vectors ahead into the thread's own slots of shared memory, over the ends of walks and rows, so that
+// neither the latency of memory nor the barriers between the walks leave the memory idle (four vectors ahead in registers,
+// begun anew for each walk: 643 us at 4096 x 128256). Four vectors a step, because the exponentials take 16 of the clocks that a
+// warp has per element and row, and everything else has to be issued beside them.
 template <typename T, int kThreads, int kDepth>
 struct Stream {
-  static constexpr int kV = Row<T>::kV;
-  static constexpr int kBytes = kDepth * kThreads * 16;
+  static constexpr int kV = Row<T>::kV, kU = 4;
+  static constexpr int kApart = kThreads * kV;  // elements from one of a thread's vectors to the next
+  static constexpr int kSlot = kThreads * 16 * kU, kBytes = kDepth * kSlot;
   uint8_t* slots;
   const mb_distill_t* d;
-  const T* at;   // the next vector to ask for
-  int64_t row;   // its row
-  int left;      // how many of this walk are still to be asked for
-  int walks;     // walks over the row after this one
-  int per_row;   // walks per row, less one
-  int slot;
+  const T* at;     // the next vector to ask for
+  const T* end;    // behind the row's last vector
+  const T* first;  // this thread's first vector of the row
+  int64_t row;     // its row
+  int walks;       // walks over the row after this one
+  int per_row;     // walks per row, less one
+  int slot;        // offset of the slot that comes next
 
-  __device__ __forceinline__ static int mine(int vecs) { return vecs > (int)threadIdx.x ? (vecs - (int)threadIdx.x + kThreads - 1) / kThreads : 0; }
-  __device__ __forceinline__ void start_walk() {
-    const T* z = reinterpret_cast<const T*>(d->logits) + row * d->stride;
-    const Row<T> shape(z, d->V);
-    at = z + shape.head + threadIdx.x * (int64_t)kV;
-    left = mine(shape.vecs);
-  }
+  // the first live row from `row` on that has vectors for this thread
   __device__ __forceinline__ void seek() {
-    while (row < d->rows && !d->live[row]) row += gridDim.x;
-    if (row < d->rows) {
+    for (; row < d->rows; row += gridDim.x) {
+      if (!d->live[row]) continue;
+      const T* z = reinterpret_cast<const T*>(d->logits) + row * d->stride;
+      const Row<T> shape(z, d->V);
+      if ((int)threadIdx.x >= shape.vecs) continue;
+      end = z + shape.head + shape.vecs * (int64_t)kV;
+      first = at = z + shape.head + threadIdx.x * (int64_t)kV;
       walks = per_row;
-      start_walk();
+      return;
     }
+    at = end = nullptr;
   }
-  __device__ __forceinline__ void begin(uint8_t* smem, const mb_distill_t& args, int64_t first, bool twice) {
+  __device__ __forceinline__ void begin(uint8_t* smem, const mb_distill_t& args, int64_t from, bool twice) {
     slots = smem + threadIdx.x * 16;
     d = &args;
-    row = first;
-    left = 0;
+    row = from;
     per_row = twice;
     slot = 0;
     seek();
 #pragma unroll 1
-    for (int i = 0; i < kDepth; ++i) ask(i);
+    for (int i = 0; i < kDepth; ++i) ask(i * kSlot);
   }
   __device__ __forceinline__ void ask(int into) {
-    while (left == 0 && row < d->rows) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slots + into);
+    if (at + (kU - 1) * kApart < end) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * kThreads * 16), "l"(at + u * kApart) : "memory");
+      at += kU * kApart;
+    } else if (at < end) {
+#pragma unroll 1
+      for (int u = 0; u < kU && at < end; ++u, at += kApart)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * kThreads * 16), "l"(at) : "memory");
+    }
+    if (at >= end && at) {
       if (walks > 0) {
         --walks;
-        start_walk();
-        if (left == 0) walks = 0;  // a row without vectors for this thread
+        at = first;
       } else {
         row += gridDim.x;
         seek();
       }
     }
-    if (left > 0) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slots + into * kThreads * 16)), "l"(at)
-                   : "memory");
-      at += kThreads * kV;
-      --left;
-    }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // f(vector, its index in the row) for this thread's vectors of one walk
-  template <typename F>
-  __device__ __forceinline__ void each(int vecs, F f) {
-    for (int i = threadIdx.x; i < vecs; i += kThreads) {
+  // whole(vectors, index of the first) for each full step of one walk over this thread's vectors, single(vector, index) for the
+  // vectors of an unfinished last step
+  template <typename F, typename G>
+  __device__ __forceinline__ void each(int vecs, F whole, G single) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < vecs; i += kU * kThreads) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-      const Pack<T, kV> v = *reinterpret_cast<const Pack<T, kV>*>(slots + slot * kThreads * 16);
-      float x[kV];
-      unpack<T, kV>(v, x);
-      f(v, x, i);
-      // the vector's values have been used, so its slot is free
+      const Pack<T, kV>* from = reinterpret_cast<const Pack<T, kV>*>(slots + slot);
+      if (i + (kU - 1) * kThreads < vecs) {
+        Pack<T, kV> v[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) v[u] = from[u * kThreads];
+        whole(v, i);
+      } else {
+#pragma unroll 1
+        for (int j = i; j < vecs; j += kThreads) single(from[j - i], j);
+      }
+      // the vectors' values have been used, so their slot is free
       ask(slot);
-      if (++slot == kDepth) slot = 0;
+      slot += kSlot;
+      if (slot == kBytes) slot = 0;
     }
   }
 };
@@ -305,9 +324,12 @@ __device__ __forceinline__ void row_gradient(const Row<T>& row, const T* z, T* g
     const int c = row.edge_column(e);
     g[c] = from_f32<T>(slope(to_f32(z[c])));
   }
-  stream.each(row.vecs, [&](const Pack<T, kV>&, float* f, int i) {
+  T* out = g + row.head;
+  auto put = [&](const Pack<T, kV>& v, int i) {
+    float f[kV];
+    unpack<T, kV>(v, f);
     slope.template all<kV>(f);
-    T* to = g + row.head + i * (int64_t)kV;
+    T* to = out + i * (int64_t)kV;
     if (same) {
       const Pack<T, kV> o = pack<T, kV>(f);
       __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&o));
@@ -315,7 +337,14 @@ __device__ __forceinline__ void row_gradient(const Row<T>& row, const T* z, T* g
 #pragma unroll
       for (int k = 0; k < kV; ++k) to[k] = from_f32<T>(f[k]);
     }
-  });
+  };
+  stream.each(
+      row.vecs,
+      [&](const Pack<T, kV>(&v)[S::kU], int i) {
+#pragma unroll
+        for (int u = 0; u < S::kU; ++u) put(v[u], i + u * kThreads);
+      },
+      put);
 }
 template <typename T, int kThreads>
 __device__ __forceinline__ void row_zeros(T* g, int V) {
@@ -361,8 +390,8 @@ __device__ __forceinline__ void stage_entries(const mb_distill_t& d, int64_t r, 
   }
 }
 
-// vectors ahead: 80 KB per CTA of 512 threads, two CTAs per SM; 8 KB per CTA of 128, up to eight
-constexpr int depth_for(int threads) { return threads > 128 ? 10 : 4; }
+// steps ahead: 96 KB per CTA of 512 threads, two CTAs per SM; 16 KB per CTA of 128, up to eight
+constexpr int depth_for(int threads) { return threads > 128 ? 3 : 2; }
 
 // kTwo: the two terms need different exponentials (a hard term, and tau is not 1)
 template <typename T, int kThreads, bool kTwo>
@@ -398,21 +427,33 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       if (my_p != 0.f) my_z = to_f32(z[id_at(d, r * d.K + threadIdx.x)]);
     }
     Running<kTwo> run(inv_tau);
-    stream.each(row.vecs, [&](const Pack<T, kV>& v, const float* f, int) {
-      run.raise(largest(v, f));
-      run.template add<kV>(f);
-    });
-    for (int e = threadIdx.x; e < row.edge; e += kThreads) {
-      const float f = to_f32(z[row.edge_column(e)]);
-      run.raise(f);
-      run.template add<1>(&f);
-    }
+    using In = decltype(stream);
+    stream.each(
+        row.vecs,
+        [&](const Pack<T, kV>(&v)[In::kU], int) {
+          run.raise(largest(v));
+#pragma unroll
+          for (int u = 0; u < In::kU; ++u) {
+            float f[kV];
+            unpack<T, kV>(v[u], f);
+            run.template add<kV>(f);
+          }
+        },
+        [&](const Pack<T, kV>& v, int) {
+          const Pack<T, kV> one[1] = {v};
+          run.raise(largest(one));
+          float f[kV];
+          unpack<T, kV>(v, f);
+          run.template add<kV>(f);
+        });
+    for (int e = threadIdx.x; e < row.edge; e += kThreads) run.add_one(to_f32(z[row.edge_column(e)]));
     // (max, sums) of the warp, then of the CTA: one barrier
     float m = warp_reduce_max(run.m);
-    float st = warp_reduce_sum(run.st * exp2_fast((run.m - m) * run.c));
-    float s1 = kTwo ? warp_reduce_sum(run.s1 * exp2_fast((run.m - m) * 1.4426950409f)) : 0.f;
+    const float2 own = split(run.st), own1 = split(run.s1);
+    float st = warp_reduce_sum((own.x + own.y) * exp2_fast((run.m - m) * run.c));
+    float s1 = kTwo ? warp_reduce_sum((own1.x + own1.y) * exp2_fast((run.m - m) * kLog2e)) : 0.f;
     // a warp that saw nothing but -inf has NaN here; it counts with nothing, unless it really saw NaN
-    if (m == -INFINITY && warp_reduce_sum(run.st) == 0.f) st = s1 = 0.f;
+    if (m == -INFINITY && warp_reduce_sum(own.x + own.y) == 0.f) st = s1 = 0.f;
     if (lane == 0) {
       red[0][warp] = m;
       red[1][warp] = st;
@@ -423,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     m = warp_reduce_max(wm);
     const bool mine = lane < kWarps;
     st = warp_reduce_sum(mine ? red[1][lane % kWarps] * exp2_fast((wm - m) * run.c) : 0.f);
-    s1 = kTwo ? warp_reduce_sum(mine ? red[2][lane % kWarps] * exp2_fast((wm - m) * 1.4426950409f) : 0.f) : st;
+    s1 = kTwo ? warp_reduce_sum(mine ? red[2][lane % kWarps] * exp2_fast((wm - m) * kLog2e) : 0.f) : st;
     const Slope<kTwo> slope{m, run.c, kTwo ? a_soft / st : (a_soft + a_hard) / st, a_hard / s1};
     // the teacher's entries against q, but for log(st)
     float ce = my_p != 0.f ? my_p * (my_z - m) * inv_tau : 0.f;
@@ -486,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     __syncthreads();  // the row before is done with the staged entries
     stage_entries<kThreads>(d, r, ids, probs);
     const float iq = d.stats[r * 3 + 1];
-    const Slope<kTwo> slope{d.stats[r * 3], 1.4426950409f / d.tau, kTwo ? a_soft * iq : (a_soft + a_hard) * iq, a_hard * d.stats[r * 3 + 2]};
+    const Slope<kTwo> slope{d.stats[r * 3], kLog2e / d.tau, kTwo ? a_soft * iq : (a_soft + a_hard) * iq, a_hard * d.stats[r * 3 + 2]};
     row_gradient<T, kThreads, kTwo>(row, z, g, stream, slope);
     __syncthreads();
     named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
@@ -519,7 +560,7 @@ inline unsigned row_ctas(int64_t rows, int V) {
 
 template <auto kKernel, int kThreads, typename... Args>
 int launch(const mb_distill_t& d, cudaStream_t s, Args... args) {
-  constexpr int smem = depth_for(kThreads) * kThreads * 16;
+  constexpr int smem = depth_for(kThreads) * kThreads * 64;
   static bool done[64];  // per kernel and device
   if (smem > 48 * 1024) {
     int device = 0;
