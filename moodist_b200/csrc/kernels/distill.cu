@@ -7,7 +7,9 @@
 // Bound by the bytes of the logits, read once, and of the gradient, written once. The gradient's scale is known in the forward
 // pass up to the incoming scalar (which is 1 unless the loss is scaled afterwards), so the forward pass writes it: a CTA walks a
 // row twice, first from memory for the maximum and the sum of exponentials, then for the gradient from L2, where the rows in
-// work (148 of 256 KB at 128256 words) stay. fp16 is the exception: its gradients would underflow before a loss scale reaches
+// work (148 of 256 KB at 128256 words) stay. A long row belongs to a cluster of two CTAs or more: two CTAs per SM, in different
+// phases of their rows, keep memory and arithmetic busy at once, and with a row each they had twice the bytes in work and read
+// 1.4 times the logits from memory. fp16 is the exception: its gradients would underflow before a loss scale reaches
 // them, so there the backward pass reads the logits again.
 // Sums and row statistics are fp32; sums have a fixed order, so the same inputs give the same bits.
 #include "kernels_api.h"
@@ -44,19 +46,27 @@ __device__ __forceinline__ bool entry(const mb_distill_t& d, int64_t i, float* t
   return *t != -INFINITY;
 }
 
-// One warp per row: the teacher's probabilities over the valid entries (0 in the others), sum p log p, whether the row counts;
-// per CTA how many rows do. Readies the ticket of the row kernel.
+// One warp per row: the teacher's probabilities over the valid entries, those of a word named several times added up at its first
+// place and 0 elsewhere (so that each word of the row is dealt with once), sum p log p, and live: 0 for a row that does not count,
+// 1, or 2 if an entry with weight names the target. Per CTA how many rows count. Readies the ticket of the row kernel.
 __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const __grid_constant__ mb_distill_t d) {
-  __shared__ int counts[kTopThreads / 32];
+  constexpr int kWarps = kTopThreads / 32;
+  __shared__ int counts[kWarps];
+  __shared__ int4 staged_ids[kWarps][kStaged / 4];  // -1: no entry
+  __shared__ float staged_w[kWarps][kStaged];       // exp((t - max) / tau)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* ids = reinterpret_cast<int*>(staged_ids[warp]);
+  float* ws = staged_w[warp];
+  const bool staged = d.K <= kStaged;
   const float inv_tau = 1.f / d.tau;
   int count = 0;
-  for (int64_t r = blockIdx.x * (int64_t)(kTopThreads / 32) + warp; r < d.rows; r += (int64_t)gridDim.x * (kTopThreads / 32)) {
+  for (int64_t r = blockIdx.x * (int64_t)kWarps + warp; r < d.rows; r += (int64_t)gridDim.x * kWarps) {
     const int64_t base = r * d.K;
-    bool counts = true;
+    int64_t target = -1;
+    bool counts_too = true;
     if (d.targets) {
-      const int64_t t = d.targets[r];
-      counts = t != d.ignore_index && t >= 0 && t < d.V;
+      target = d.targets[r];
+      counts_too = target != d.ignore_index && target >= 0 && target < d.V;
     }
     float m = -INFINITY, t;
     bool any = false;
@@ -67,34 +77,70 @@ __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const __gr
       }
     }
     m = warp_reduce_max(m);
-    const bool live = counts && __any_sync(0xffffffffu, any);
+    const bool live = counts_too && __any_sync(0xffffffffu, any);
     float s = 0.f, e = 0.f;
-    for (int k = lane; k < d.K; k += 32) {
-      float w = 0.f;
-      if (live && entry(d, base + k, &t)) {
-        t = (t - m) * inv_tau;
-        w = expf(t);
-        s += w;
-        if (!(w <= 0.f)) e += w * t;  // weight 0: t may have overflowed to -inf; NaN goes on
-      }
-      d.p[base + k] = w;
-    }
-    s = warp_reduce_sum(s);
-    e = warp_reduce_sum(e);
+    bool hit = false;
     if (live) {
-      const float inv = 1.f / s;
-      for (int k = lane; k < d.K; k += 32) d.p[base + k] *= inv;
+      __syncwarp();
+      for (int k = lane; k < d.K; k += 32) {
+        float w = 0.f;
+        const bool there = entry(d, base + k, &t);
+        if (there) {
+          t = (t - m) * inv_tau;
+          w = expf(t);
+          s += w;
+          if (!(w <= 0.f)) e += w * t;  // weight 0: t may have overflowed to -inf; NaN goes on
+        }
+        if (staged) {
+          ids[k] = there ? (int)id_at(d, base + k) : -1;
+          ws[k] = w;
+        }
+      }
+      if (staged && lane < (4 - d.K % 4) % 4) ids[d.K + lane] = -1;
+      s = warp_reduce_sum(s);
+      e = warp_reduce_sum(e);
+      __syncwarp();
     }
+    const float inv = 1.f / s;
+    for (int k = lane; k < d.K; k += 32) {
+      float p = 0.f;
+      if (live && entry(d, base + k, &t)) {
+        const int id = (int)id_at(d, base + k);
+        bool first = true;
+        p = expf((t - m) * inv_tau);
+        auto same = [&](int i, float w) {
+          if (i < k) first = false;
+          if (i > k) p += w;
+        };
+        if (staged) {
+          for (int i = 0; i < d.K; i += 4) {
+            const int4 o = staged_ids[warp][i / 4];
+            if (o.x == id) same(i, ws[i]);
+            if (o.y == id) same(i + 1, ws[i + 1]);
+            if (o.z == id) same(i + 2, ws[i + 2]);
+            if (o.w == id) same(i + 3, ws[i + 3]);
+          }
+        } else {
+          float w;
+          for (int i = 0; i < d.K; ++i)
+            if (entry(d, base + i, &w) && id_at(d, base + i) == id) same(i, expf((w - m) * inv_tau));
+        }
+        p = first ? p * inv : 0.f;
+        hit |= p != 0.f && id == target;
+      }
+      d.p[base + k] = p;
+    }
+    hit = __any_sync(0xffffffffu, hit);
     count += live;
     if (lane == 0) {
-      d.live[r] = live;
-      d.entropy[r] = live ? e / s - logf(s) : 0.f;
+      d.live[r] = live ? (hit ? 2 : 1) : 0;
+      d.entropy[r] = live ? e * inv - logf(s) : 0.f;
     }
   }
   if (lane == 0) counts[warp] = count;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kTopThreads / 32; ++w) count += counts[w];
+    for (int w = 1; w < kWarps; ++w) count += counts[w];
     d.counts[blockIdx.x] = count;
     if (blockIdx.x == 0) d.counts[kTopCtas] = 0;
   }
@@ -223,6 +269,20 @@ struct Slope {
   }
 };
 
+// A CTA's part of every row: columns [from, from + count)
+struct Part {
+  int rank, parts, from, count;
+  __device__ __forceinline__ Part(int n, int V) {
+    parts = n;
+    rank = blockIdx.x % n;
+    const int each = ((V + n - 1) / n + 63) / 64 * 64;
+    from = min(rank * each, V);
+    count = min(each, V - from);
+  }
+  __device__ __forceinline__ int64_t first_row() const { return blockIdx.x / parts; }
+  __device__ __forceinline__ int64_t step() const { return gridDim.x / parts; }
+};
+
 // The vectors that a thread is going to read, in order: those of its rows, each row once or, with the gradient, twice. They travel
 // kDepth steps of four vectors ahead into the thread's own slots of shared memory, over the ends of walks and rows, so that
 // neither the latency of memory nor the barriers between the walks leave the memory idle (four vectors ahead in registers,
@@ -235,6 +295,7 @@ struct Stream {
   static constexpr int kSlot = kThreads * 16 * kU, kBytes = kDepth * kSlot;
   uint8_t* slots;
   const mb_distill_t* d;
+  const Part* part;
   const T* at;     // the next vector to ask for
   const T* end;    // behind the row's last vector
   const T* first;  // this thread's first vector of the row
@@ -242,13 +303,16 @@ struct Stream {
   int walks;       // walks over the row after this one
   int per_row;     // walks per row, less one
   int slot;        // offset of the slot that comes next
+  int live;        // whether `row` counts, known before it is needed
 
   // the first live row from `row` on that has vectors for this thread
   __device__ __forceinline__ void seek() {
-    for (; row < d->rows; row += gridDim.x) {
-      if (!d->live[row]) continue;
-      const T* z = reinterpret_cast<const T*>(d->logits) + row * d->stride;
-      const Row<T> shape(z, d->V);
+    for (; row < d->rows; row += part->step()) {
+      const int now = live;
+      if (row + part->step() < d->rows) live = d->live[row + part->step()];
+      if (!now) continue;
+      const T* z = reinterpret_cast<const T*>(d->logits) + row * d->stride + part->from;
+      const Row<T> shape(z, part->count);
       if ((int)threadIdx.x >= shape.vecs) continue;
       end = z + shape.head + shape.vecs * (int64_t)kV;
       first = at = z + shape.head + threadIdx.x * (int64_t)kV;
@@ -257,12 +321,14 @@ struct Stream {
     }
     at = end = nullptr;
   }
-  __device__ __forceinline__ void begin(uint8_t* smem, const mb_distill_t& args, int64_t from, bool twice) {
+  __device__ __forceinline__ void begin(uint8_t* smem, const mb_distill_t& args, const Part& mine, bool twice) {
     slots = smem + threadIdx.x * 16;
     d = &args;
-    row = from;
+    part = &mine;
+    row = mine.first_row();
     per_row = twice;
     slot = 0;
+    live = row < args.rows ? args.live[row] : 0;
     seek();
 #pragma unroll 1
     for (int i = 0; i < kDepth; ++i) ask(i * kSlot);
@@ -284,7 +350,7 @@ struct Stream {
         --walks;
         at = first;
       } else {
-        row += gridDim.x;
+        row += part->step();
         seek();
       }
     }
@@ -354,88 +420,130 @@ __device__ __forceinline__ void row_zeros(T* g, int V) {
   for (int i = threadIdx.x; i < row.vecs; i += kThreads) *reinterpret_cast<uint4*>(g + row.head + i * (int64_t)kV) = make_uint4(0, 0, 0, 0);
 }
 
-// The places that the teacher or the target names, each written once, by the warp of the first entry that names it: a warp per
-// entry, whose lanes look through the others. The rest of the row's gradient has been written and a barrier passed.
+// The words that the teacher or the target names. Thread k deals with the teacher's entry k (and kThreads more at a time), whose
+// probability the teacher kernel has merged over the row: it subtracts it from the gradient that the walk has written there.
+// The target goes with its entry, or alone when the teacher does not name it. Only places of this CTA's part are written, after
+// a barrier behind the walk.
 template <typename T, int kThreads, bool kTwo>
-__device__ __forceinline__ void named_places(const mb_distill_t& d, int64_t r, const T* z, T* g, const Slope<kTwo>& slope, float a_soft,
-                                             float a_hard, const int* ids, const float* p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = a_hard != 0.f ? d.targets[r] : -1;
-  const bool staged = d.K <= kStaged;
-  for (int k = threadIdx.x >> 5; k <= d.K; k += kThreads / 32) {
-    const int64_t j = k == d.K ? t : staged ? (int64_t)ids[k] : id_at(d, r * d.K + k);
-    if (j < 0 || j >= d.V) continue;
-    bool earlier = false;
-    float sum = 0.f;
-    for (int i = lane; i < d.K; i += 32) {
-      if ((staged ? (int64_t)ids[i] : id_at(d, r * d.K + i)) == j) {
-        earlier |= i < k;
-        sum += staged ? p[i] : d.p[r * d.K + i];
-      }
-    }
-    if (__any_sync(0xffffffffu, earlier)) continue;
-    sum = warp_reduce_sum(sum);
-    if (lane == 0) g[j] = from_f32<T>(slope(to_f32(z[j])) - sum * a_soft - (j == t ? a_hard : 0.f));
-  }
+__device__ __forceinline__ void named_place(const mb_distill_t& d, int64_t r, T* g, const Part& part, const Slope<kTwo>& slope, float a_soft,
+                                            float a_hard, int64_t t, int id, float p, float z) {
+  if (p != 0.f && id >= part.from && id < part.from + part.count) g[id] = from_f32<T>(slope(z) - p * a_soft - (id == t ? a_hard : 0.f));
 }
-
-// the row's teacher entries in shared memory, ids outside the vocabulary as -1
-template <int kThreads>
-__device__ __forceinline__ void stage_entries(const mb_distill_t& d, int64_t r, int* ids, float* p) {
-  if (d.K > kStaged) return;
-  for (int k = threadIdx.x; k < d.K; k += kThreads) {
-    const int64_t id = id_at(d, r * d.K + k);
-    ids[k] = id >= 0 && id < d.V ? (int)id : -1;
-    p[k] = d.p[r * d.K + k];
+template <typename T, int kThreads, bool kTwo>
+__device__ __forceinline__ void other_places(const mb_distill_t& d, int64_t r, const T* z, T* g, const Part& part, const Slope<kTwo>& slope,
+                                             float a_soft, float a_hard, int64_t t, int live) {
+  for (int k = threadIdx.x + kThreads; k < d.K; k += kThreads) {
+    const float p = d.p[r * d.K + k];
+    if (p != 0.f) {
+      const int id = (int)id_at(d, r * d.K + k);
+      named_place<T, kThreads, kTwo>(d, r, g, part, slope, a_soft, a_hard, t, id, p, to_f32(z[id]));
+    }
   }
+  if (live == 1 && threadIdx.x == kThreads - 1 && t >= part.from && t < part.from + part.count)
+    g[t] = from_f32<T>(slope(to_f32(z[t])) - a_hard);
 }
 
 // steps ahead: 96 KB per CTA of 512 threads, two CTAs per SM; 16 KB per CTA of 128, up to eight
 constexpr int depth_for(int threads) { return threads > 128 ? 3 : 2; }
 
-// kTwo: the two terms need different exponentials (a hard term, and tau is not 1)
+__device__ __forceinline__ float ld_cluster(const float* p, int cta) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+// every thread of every CTA of the cluster
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// What is left of a row when its walk is over: its named places and its loss wait for the next barrier, which is that of the
+// row after.
+template <bool kTwo>
+struct Unfinished {
+  int64_t r = -1;
+  Slope<kTwo> slope;
+  int id, live;
+  float p, z, st, s1;
+};
+
+// kTwo: the two terms need different exponentials (a hard term, and tau is not 1). The grid is clusters of `parts` CTAs, one row
+// at a time per cluster, one barrier per row.
 template <typename T, int kThreads, bool kTwo>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
-    distill_row_kernel(const __grid_constant__ mb_distill_t d, T* __restrict__ grad, int64_t grad_stride) {
+    distill_row_kernel(const __grid_constant__ mb_distill_t d, int parts, T* __restrict__ grad, int64_t grad_stride) {
   constexpr int kV = Row<T>::kV, kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float red[4][kWarps];
-  __shared__ int ids[kStaged];
-  __shared__ float probs[kStaged];
+  __shared__ float red[2][4][kWarps];  // by row parity: a peer may still read the row before's
   __shared__ int shared_count;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float inv_tau = 1.f / d.tau;
   const float factor = row_factor<kThreads>(d, &shared_count);
   const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
-  Stream<T, kThreads, depth_for(kThreads)> stream;
-  stream.begin(ring, d, blockIdx.x, grad != nullptr);
-  for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
+  const Part part(parts, d.V);
+  using In = Stream<T, kThreads, depth_for(kThreads)>;
+  In stream;
+  stream.begin(ring, d, part, grad != nullptr);
+  int parity = 0;
+  Unfinished<kTwo> u;
+  auto finish = [&](int from) {
+    const T* z = reinterpret_cast<const T*>(d.logits) + u.r * d.stride;
+    const int64_t t = d.hard > 0.f ? d.targets[u.r] : -1;
+    if (grad) {
+      T* g = grad + u.r * grad_stride;
+      named_place<T, kThreads, kTwo>(d, u.r, g, part, u.slope, a_soft, a_hard, t, u.id, u.p, u.z);
+      if (d.K > kThreads || (t >= 0 && u.live == 1)) other_places<T, kThreads, kTwo>(d, u.r, z, g, part, u.slope, a_soft, a_hard, t, u.live);
+    }
+    if (warp == 0 && part.rank == 0) {
+      const float ce = warp_reduce_sum(lane < kWarps ? red[from][3][lane % kWarps] : 0.f);
+      if (lane == 0) {
+        const float m = u.slope.m;
+        d.stats[u.r * 3] = m;
+        d.stats[u.r * 3 + 1] = 1.f / u.st;
+        d.stats[u.r * 3 + 2] = 1.f / u.s1;
+        // the probabilities sum to 1, so log(st) stands outside the sum
+        float l = d.hard < 1.f ? (1.f - d.hard) * d.tau * d.tau * (d.entropy[u.r] - ce + logf(u.st)) : 0.f;
+        if (d.hard > 0.f) l += d.hard * (logf(u.s1) + m - to_f32(z[t]));
+        d.row_loss[u.r] = l;
+      }
+    }
+  };
+  // this thread's entry of the next row and whether that row counts, asked for a row ahead
+  float next_p = 0.f;
+  int next_id = 0, next_live = 0;
+  auto peek = [&](int64_t r) {
+    if (r >= d.rows) return;
+    next_live = d.live[r];
+    if (threadIdx.x < d.K) {
+      next_p = d.p[r * d.K + threadIdx.x];
+      next_id = (int)id_at(d, r * d.K + threadIdx.x);
+    }
+  };
+  peek(part.first_row());
+  for (int64_t r = part.first_row(); r < d.rows; r += part.step()) {
     const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
     T* g = grad + r * grad_stride;
-    if (!d.live[r]) {
-      if (threadIdx.x == 0) d.row_loss[r] = 0.f;
-      if (grad) row_zeros<T, kThreads>(g, d.V);
+    const int live = next_live, my_id = next_id;
+    const float my_p = next_p;
+    float my_z = 0.f;
+    if (live && my_p != 0.f) my_z = to_f32(z[my_id]);
+    peek(r + part.step());
+    if (!live) {
+      if (threadIdx.x == 0 && part.rank == 0) d.row_loss[r] = 0.f;
+      if (grad) row_zeros<T, kThreads>(g + part.from, part.count);
       continue;
     }
-    const Row<T> row(z, d.V);
-    __syncthreads();  // the row before is done with the staged entries
-    stage_entries<kThreads>(d, r, ids, probs);
-    // this thread's teacher entry, on its way while the row is read
-    float my_p = 0.f, my_z = 0.f;
-    if (threadIdx.x < d.K) {
-      my_p = d.p[r * d.K + threadIdx.x];
-      if (my_p != 0.f) my_z = to_f32(z[id_at(d, r * d.K + threadIdx.x)]);
-    }
+    const Row<T> row(z + part.from, part.count);
     Running<kTwo> run(inv_tau);
-    using In = decltype(stream);
     stream.each(
         row.vecs,
         [&](const Pack<T, kV>(&v)[In::kU], int) {
           run.raise(largest(v));
 #pragma unroll
-          for (int u = 0; u < In::kU; ++u) {
+          for (int i = 0; i < In::kU; ++i) {
             float f[kV];
-            unpack<T, kV>(v[u], f);
+            unpack<T, kV>(v[i], f);
             run.template add<kV>(f);
           }
         },
@@ -446,8 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           unpack<T, kV>(v, f);
           run.template add<kV>(f);
         });
-    for (int e = threadIdx.x; e < row.edge; e += kThreads) run.add_one(to_f32(z[row.edge_column(e)]));
-    // (max, sums) of the warp, then of the CTA: one barrier
+    for (int e = threadIdx.x; e < row.edge; e += kThreads) run.add_one(to_f32(z[part.from + row.edge_column(e)]));
+    // (max, sums) of the warp, then of the cluster: one barrier
     float m = warp_reduce_max(run.m);
     const float2 own = split(run.st), own1 = split(run.s1);
     float st = warp_reduce_sum((own.x + own.y) * exp2_fast((run.m - m) * run.c));
@@ -455,41 +563,55 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     // a warp that saw nothing but -inf has NaN here; it counts with nothing, unless it really saw NaN
     if (m == -INFINITY && warp_reduce_sum(own.x + own.y) == 0.f) st = s1 = 0.f;
     if (lane == 0) {
-      red[0][warp] = m;
-      red[1][warp] = st;
-      red[2][warp] = s1;
+      red[parity][0][warp] = m;
+      red[parity][1][warp] = st;
+      red[parity][2][warp] = s1;
     }
-    __syncthreads();
-    const float wm = red[0][lane % kWarps];
-    m = warp_reduce_max(wm);
-    const bool mine = lane < kWarps;
-    st = warp_reduce_sum(mine ? red[1][lane % kWarps] * exp2_fast((wm - m) * run.c) : 0.f);
-    s1 = kTwo ? warp_reduce_sum(mine ? red[2][lane % kWarps] * exp2_fast((wm - m) * kLog2e) : 0.f) : st;
-    const Slope<kTwo> slope{m, run.c, kTwo ? a_soft / st : (a_soft + a_hard) / st, a_hard / s1};
-    // the teacher's entries against q, but for log(st)
-    float ce = my_p != 0.f ? my_p * (my_z - m) * inv_tau : 0.f;
-    for (int k = threadIdx.x + kThreads; k < d.K; k += kThreads) {
-      const float p = d.p[r * d.K + k];
-      if (p != 0.f) ce += p * (to_f32(z[id_at(d, r * d.K + k)]) - m) * inv_tau;
-    }
-    ce = warp_reduce_sum(ce);
-    if (lane == 0) red[3][warp] = ce;
-    if (grad) row_gradient<T, kThreads, kTwo>(row, z, g, stream, slope);
-    __syncthreads();
-    if (grad) named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
-    if (warp == 0) {
-      ce = warp_reduce_sum(mine ? red[3][lane % kWarps] : 0.f);
-      if (lane == 0) {
-        d.stats[r * 3] = m;
-        d.stats[r * 3 + 1] = 1.f / st;
-        d.stats[r * 3 + 2] = 1.f / s1;
-        // the probabilities sum to 1, so log(st) stands outside the sum
-        float l = d.hard < 1.f ? (1.f - d.hard) * d.tau * d.tau * (d.entropy[r] - ce + logf(st)) : 0.f;
-        if (d.hard > 0.f) l += d.hard * (logf(s1) + m - to_f32(z[d.targets[r]]));
-        d.row_loss[r] = l;
+    if (parts > 1)
+      cluster_barrier();
+    else
+      __syncthreads();
+    {
+      float wm = -INFINITY, wt = 0.f, w1 = 0.f;
+      m = -INFINITY;
+      for (int i = lane; i < parts * kWarps; i += 32) {
+        const float om = ld_cluster(&red[parity][0][i % kWarps], i / kWarps), ot = ld_cluster(&red[parity][1][i % kWarps], i / kWarps);
+        const float o1 = kTwo ? ld_cluster(&red[parity][2][i % kWarps], i / kWarps) : 0.f;
+        const float nm = fmaxf(wm, om);
+        // (a sum of 0 goes with -inf: nothing of it counts)
+        wt = (wt == 0.f ? 0.f : wt * exp2_fast((wm - nm) * run.c)) + (ot == 0.f ? 0.f : ot * exp2_fast((om - nm) * run.c));
+        if (kTwo) w1 = (w1 == 0.f ? 0.f : w1 * exp2_fast((wm - nm) * kLog2e)) + (o1 == 0.f ? 0.f : o1 * exp2_fast((om - nm) * kLog2e));
+        wm = nm;
       }
+      m = warp_reduce_max(wm);
+      st = warp_reduce_sum(wt * exp2_fast((wm - m) * run.c));
+      s1 = kTwo ? warp_reduce_sum(w1 * exp2_fast((wm - m) * kLog2e)) : st;
     }
+    if (u.r >= 0) finish(parity ^ 1);
+    u.r = r;
+    u.slope = Slope<kTwo>{m, run.c, kTwo ? a_soft / st : (a_soft + a_hard) / st, a_hard / s1};
+    u.id = my_id;
+    u.live = live;
+    u.p = my_p;
+    u.z = my_z;
+    u.st = st;
+    u.s1 = s1;
+    if (part.rank == 0) {
+      // the teacher's entries against q, but for log(st)
+      float ce = my_p != 0.f ? my_p * (my_z - m) * inv_tau : 0.f;
+      for (int k = threadIdx.x + kThreads; k < d.K; k += kThreads) {
+        const float p = d.p[r * d.K + k];
+        if (p != 0.f) ce += p * (to_f32(z[id_at(d, r * d.K + k)]) - m) * inv_tau;
+      }
+      ce = warp_reduce_sum(ce);
+      if (lane == 0) red[parity][3][warp] = ce;
+    }
+    if (grad) row_gradient<T, kThreads, kTwo>(row, z + part.from, g + part.from, stream, u.slope);
+    parity ^= 1;
   }
+  __syncthreads();
+  if (u.r >= 0) finish(parity ^ 1);
+  if (parts > 1) cluster_barrier();  // the peers no longer read this CTA's sums
   // the last CTA to get here adds the row losses up, in a fixed order
   __shared__ bool last;
   __threadfence();
@@ -500,37 +622,44 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __threadfence();
   float s = 0.f;
   for (int64_t r = threadIdx.x; r < d.rows; r += kThreads) s += __ldcg(d.row_loss + r);
-  s = block_reduce_sum<kThreads>(s, red[0]);
+  s = block_reduce_sum<kThreads>(s, red[0][0]);
   if (threadIdx.x == 0) d.loss[0] = s * factor;
 }
 
 // the backward pass on its own: the logits once more
 template <typename T, int kThreads, bool kTwo>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
-    distill_grad_kernel(const __grid_constant__ mb_distill_t d, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
+    distill_grad_kernel(const __grid_constant__ mb_distill_t d, int parts, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ int ids[kStaged];
-  __shared__ float probs[kStaged];
   __shared__ int shared_count;
   const float factor = row_factor<kThreads>(d, &shared_count) * gout[0];
   const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
+  const Part part(parts, d.V);
   Stream<T, kThreads, depth_for(kThreads)> stream;
-  stream.begin(ring, d, blockIdx.x, false);
-  for (int64_t r = blockIdx.x; r < d.rows; r += gridDim.x) {
+  stream.begin(ring, d, part, false);
+  for (int64_t r = part.first_row(); r < d.rows; r += part.step()) {
     const T* z = reinterpret_cast<const T*>(d.logits) + r * d.stride;
     T* g = grad + r * grad_stride;
-    if (!d.live[r]) {
-      row_zeros<T, kThreads>(g, d.V);
+    const int live = d.live[r];
+    if (!live) {
+      row_zeros<T, kThreads>(g + part.from, part.count);
       continue;
     }
-    const Row<T> row(z, d.V);
-    __syncthreads();  // the row before is done with the staged entries
-    stage_entries<kThreads>(d, r, ids, probs);
+    const Row<T> row(z + part.from, part.count);
+    float my_p = 0.f, my_z = 0.f;
+    int my_id = 0;
+    if (threadIdx.x < d.K) {
+      my_p = d.p[r * d.K + threadIdx.x];
+      my_id = (int)id_at(d, r * d.K + threadIdx.x);
+      if (my_p != 0.f) my_z = to_f32(z[my_id]);
+    }
+    const int64_t t = d.hard > 0.f ? d.targets[r] : -1;
     const float iq = d.stats[r * 3 + 1];
     const Slope<kTwo> slope{d.stats[r * 3], kLog2e / d.tau, kTwo ? a_soft * iq : (a_soft + a_hard) * iq, a_hard * d.stats[r * 3 + 2]};
-    row_gradient<T, kThreads, kTwo>(row, z, g, stream, slope);
+    row_gradient<T, kThreads, kTwo>(row, z + part.from, g + part.from, stream, slope);
     __syncthreads();
-    named_places<T, kThreads, kTwo>(d, r, z, g, slope, a_soft, a_hard, ids, probs);
+    named_place<T, kThreads, kTwo>(d, r, g, part, slope, a_soft, a_hard, t, my_id, my_p, my_z);
+    if (d.K > kThreads || (t >= 0 && live == 1)) other_places<T, kThreads, kTwo>(d, r, z, g, part, slope, a_soft, a_hard, t, live);
   }
 }
 
@@ -550,15 +679,22 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_
   for (int64_t i = vecs * kV + blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) x[i] = from_f32<T>(to_f32(x[i]) * f);
 }
 
-// One CTA per row at a time. Long rows get LONG threads and 1024 / LONG CTAs per SM, so that the rows in work fit L2 between
-// their two walks; up to 8192 words 128 threads hold a row's latency and many CTAs share an SM.
+// Rows above 8192 words: clusters of 512-thread CTAs, two CTAs per SM; two to a row, and four or eight where there are too few
+// rows to fill the GPU otherwise and the parts stay above 4096 words. Shorter rows: a CTA of 128 threads each, many per SM.
 constexpr int kLongRow = 8192, kLongThreads = 512;
+inline int row_parts(int64_t rows, int V) {
+  if (V <= kLongRow) return 1;
+  int n = 2;
+  while (n < 8 && rows * n * 2 <= kSms * 2 && V / (n * 2) >= 4096) n *= 2;
+  return n;
+}
 inline unsigned row_ctas(int64_t rows, int V) {
-  const int64_t most = V > kLongRow ? kSms * (1024 / kLongThreads) : kSms * 8;
-  return (unsigned)(rows < most ? rows : most);
+  const int parts = row_parts(rows, V);
+  const int64_t most = V > kLongRow ? kSms * (1024 / kLongThreads) / parts : kSms * 8;
+  return (unsigned)(rows < most ? rows : most) * parts;
 }
 
-template <auto kKernel, int kThreads, typename... Args>
+template <auto kKernel, int kThreads, bool kCluster, typename... Args>
 int launch(const mb_distill_t& d, cudaStream_t s, Args... args) {
   constexpr int smem = depth_for(kThreads) * kThreads * 64;
   static bool done[64];  // per kernel and device
@@ -568,17 +704,28 @@ int launch(const mb_distill_t& d, cudaStream_t s, Args... args) {
     if (!done[device] && cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return MB_ERR_LAUNCH;
     done[device] = true;
   }
-  kKernel<<<row_ctas(d.rows, d.V), kThreads, smem, s>>>(d, args...);
-  return check_launch();
+  const int parts = row_parts(d.rows, d.V);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(row_ctas(d.rows, d.V), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = kCluster && parts > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kKernel, d, parts, args...) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
 template <typename T, int kThreads, bool kTwo>
 int fwd_with(const mb_distill_t& d, void* grad, int64_t grad_stride, cudaStream_t s) {
-  return launch<distill_row_kernel<T, kThreads, kTwo>, kThreads>(d, s, (T*)grad, grad_stride);
+  return launch<distill_row_kernel<T, kThreads, kTwo>, kThreads, true>(d, s, (T*)grad, grad_stride);
 }
 template <typename T, int kThreads, bool kTwo>
 int bwd_with(const mb_distill_t& d, const float* gout, void* grad, int64_t grad_stride, cudaStream_t s) {
-  return launch<distill_grad_kernel<T, kThreads, kTwo>, kThreads>(d, s, gout, (T*)grad, grad_stride);
+  return launch<distill_grad_kernel<T, kThreads, kTwo>, kThreads, false>(d, s, gout, (T*)grad, grad_stride);
 }
 template <typename T>
 int fwd(const mb_distill_t& d, void* grad, int64_t grad_stride, cudaStream_t s) {

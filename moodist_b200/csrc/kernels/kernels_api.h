@@ -252,7 +252,7 @@ typedef struct {
   int64_t ignore_index;
   float tau, hard, scale;
   int mean;        // 1: over the rows that take part, 0: sum
-  float* p;         // scratch [rows, K]: the teacher's probabilities
+  float* p;         // scratch [rows, K]: the teacher's probabilities, merged per word of a row
   float* entropy;   // scratch [rows]: sum_k p_k log p_k
   int* live;        // scratch [rows]
   float* stats;     // [rows, 3]: max, 1 / sum exp((z - max) / tau), 1 / sum exp(z - max)
