@@ -7,12 +7,13 @@
 // Bound by the bytes of the logits, read once, and of the gradient, written once. The gradient's scale is known in the forward
 // pass up to the incoming scalar (which is 1 unless the loss is scaled afterwards), so the forward pass writes it: a CTA walks a
 // row twice, first from memory for the maximum and the sum of exponentials, then for the gradient from L2, where the rows in
-// work (148 of 256 KB at 128256 words) stay. A long row belongs to a cluster of two CTAs or more: two CTAs per SM, in different
-// phases of their rows, keep memory and arithmetic busy at once, and with a row each they had twice the bytes in work and read
-// 1.4 times the logits from memory. fp16 is the exception: its gradients would underflow before a loss scale reaches
+// work (148 of 256 KB at 128256 words, one CTA of 1024 threads per SM) stay. Two CTAs per SM with a row each read 1.4 times the
+// logits from memory, and two that share rows as a cluster pay for their barriers: 520 and 474 us at 4096 x 128256 bf16
+// against 458. Where there are fewer rows than SMs, clusters do share them. fp16 is the exception: its gradients would underflow before a loss scale reaches
 // them, so there the backward pass reads the logits again.
 // Sums and row statistics are fp32; sums have a fixed order, so the same inputs give the same bits.
 #include "kernels_api.h"
+#include "ptx.cuh"
 #include "vec_io.cuh"
 
 #define MB_STREAM(s) reinterpret_cast<cudaStream_t>(s)
@@ -27,7 +28,7 @@ constexpr int kSms = 148;
 constexpr int kTopThreads = 128;
 constexpr int kTopCtas = kSms * 8;
 static_assert(kTopCtas + 1 <= MB_DISTILL_COUNTS, "one count per CTA and a ticket");
-constexpr int kStaged = 1024;  // teacher entries of a row that fit shared memory
+constexpr int kStaged = 1024;  // teacher entries of a row that are compared in shared memory
 
 __device__ __forceinline__ int64_t id_at(const mb_distill_t& d, int64_t i) {
   return d.ids_i64 ? reinterpret_cast<const int64_t*>(d.ids)[i] : (int64_t)reinterpret_cast<const int32_t*>(d.ids)[i];
@@ -51,13 +52,14 @@ __device__ __forceinline__ bool entry(const mb_distill_t& d, int64_t i, float* t
 // 1, or 2 if an entry with weight names the target. Per CTA how many rows count. Readies the ticket of the row kernel.
 __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const __grid_constant__ mb_distill_t d) {
   constexpr int kWarps = kTopThreads / 32;
+  extern __shared__ int4 entries[];  // per warp: the ids (-1: no entry), then exp((t - max) / tau)
   __shared__ int counts[kWarps];
-  __shared__ int4 staged_ids[kWarps][kStaged / 4];  // -1: no entry
-  __shared__ float staged_w[kWarps][kStaged];       // exp((t - max) / tau)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* ids = reinterpret_cast<int*>(staged_ids[warp]);
-  float* ws = staged_w[warp];
   const bool staged = d.K <= kStaged;
+  const int quads = (d.K + 3) / 4;
+  const int4* id_quads = entries + warp * 2 * quads;
+  int* ids = reinterpret_cast<int*>(entries + warp * 2 * quads);
+  float* ws = reinterpret_cast<float*>(ids + 4 * quads);
   const float inv_tau = 1.f / d.tau;
   int count = 0;
   for (int64_t r = blockIdx.x * (int64_t)kWarps + warp; r < d.rows; r += (int64_t)gridDim.x * kWarps) {
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const __gr
         };
         if (staged) {
           for (int i = 0; i < d.K; i += 4) {
-            const int4 o = staged_ids[warp][i / 4];
+            const int4 o = id_quads[i / 4];
             if (o.x == id) same(i, ws[i]);
             if (o.y == id) same(i + 1, ws[i + 1]);
             if (o.z == id) same(i + 2, ws[i + 2]);
@@ -139,6 +141,7 @@ __global__ void __launch_bounds__(kTopThreads) distill_teacher_kernel(const __gr
   }
   if (lane == 0) counts[warp] = count;
   __syncthreads();
+  grid_release();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kWarps; ++w) count += counts[w];
     d.counts[blockIdx.x] = count;
@@ -443,7 +446,7 @@ __device__ __forceinline__ void other_places(const mb_distill_t& d, int64_t r, c
     g[t] = from_f32<T>(slope(to_f32(z[t])) - a_hard);
 }
 
-// steps ahead: 96 KB per CTA of 512 threads, two CTAs per SM; 16 KB per CTA of 128, up to eight
+// steps ahead: 192 KB per CTA of 1024 threads, one per SM; 16 KB per CTA of 128, up to eight
 constexpr int depth_for(int threads) { return threads > 128 ? 3 : 2; }
 
 __device__ __forceinline__ float ld_cluster(const float* p, int cta) {
@@ -479,6 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   __shared__ int shared_count;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float inv_tau = 1.f / d.tau;
+  grid_wait();
   const float factor = row_factor<kThreads>(d, &shared_count);
   const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
   const Part part(parts, d.V);
@@ -632,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     distill_grad_kernel(const __grid_constant__ mb_distill_t d, int parts, const float* __restrict__ gout, T* __restrict__ grad, int64_t grad_stride) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ int shared_count;
+  grid_wait();
   const float factor = row_factor<kThreads>(d, &shared_count) * gout[0];
   const float a_soft = (1.f - d.hard) * d.tau * factor, a_hard = d.hard * factor;
   const Part part(parts, d.V);
@@ -679,13 +684,12 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* __restrict__ x, int64_
   for (int64_t i = vecs * kV + blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) x[i] = from_f32<T>(to_f32(x[i]) * f);
 }
 
-// Rows above 8192 words: clusters of 512-thread CTAs, two CTAs per SM; two to a row, and four or eight where there are too few
-// rows to fill the GPU otherwise and the parts stay above 4096 words. Shorter rows: a CTA of 128 threads each, many per SM.
-constexpr int kLongRow = 8192, kLongThreads = 512;
+// Rows above 8192 words: a CTA of 1024 threads each, one per SM; a cluster of up to eight where the rows are too few to fill the
+// GPU otherwise and the parts stay above 4096 words. Shorter rows: a CTA of 128 threads each, many per SM.
+constexpr int kLongRow = 8192, kLongThreads = 1024;
 inline int row_parts(int64_t rows, int V) {
-  if (V <= kLongRow) return 1;
-  int n = 2;
-  while (n < 8 && rows * n * 2 <= kSms * 2 && V / (n * 2) >= 4096) n *= 2;
+  int n = 1;
+  while (V > kLongRow && n < 8 && rows * n * 2 <= kSms && V / (n * 2) >= 4096) n *= 2;
   return n;
 }
 inline unsigned row_ctas(int64_t rows, int V) {
@@ -706,16 +710,18 @@ int launch(const mb_distill_t& d, cudaStream_t s, Args... args) {
   }
   const int parts = row_parts(d.rows, d.V);
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.x = kCluster ? parts : 1;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(row_ctas(d.rows, d.V), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = kCluster && parts > 1 ? 1 : 0;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kKernel, d, parts, args...) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
@@ -750,7 +756,8 @@ bool sane(const mb_distill_t& d) {
 extern "C" int mb_distill_fwd(const mb_distill_t* d, void* grad, int64_t grad_stride, void* stream) {
   if (!sane(*d)) return MB_ERR_ARG;
   cudaStream_t s = MB_STREAM(stream);
-  distill_teacher_kernel<<<top_ctas(d->rows), kTopThreads, 0, s>>>(*d);
+  const int staged = d->K <= kStaged ? kTopThreads / 32 * ((d->K + 3) / 4) * 32 : 0;  // 32 KB at most
+  distill_teacher_kernel<<<top_ctas(d->rows), kTopThreads, staged, s>>>(*d);
   if (check_launch()) return MB_ERR_LAUNCH;
   switch (d->dtype) {
     case MB_BF16: return fwd<__nv_bfloat16>(*d, grad, grad_stride, s);
