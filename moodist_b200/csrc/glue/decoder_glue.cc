@@ -85,16 +85,16 @@ int weight_code(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b) {
 }
 
 at::Tensor layer_norm_run(const at::Tensor& x2, const at::Tensor& w, const at::Tensor& b, at::IntArrayRef shape, double eps,
-                          at::Tensor* mean, at::Tensor* rstd) {
+                          at::Tensor* stats) {
   const int64_t rows = x2.size(0), D = x2.size(1);
   at::Tensor y = at::empty(shape, x2.options());
-  if (mean) {
-    *mean = at::empty({rows}, x2.options().dtype(at::kFloat));
-    *rstd = at::empty({rows}, x2.options().dtype(at::kFloat));
+  float* mean = nullptr;
+  if (stats) {
+    *stats = at::empty({2, rows}, x2.options().dtype(at::kFloat));  // means, then 1 / deviations
+    mean = stats->data_ptr<float>();
   }
-  run(mb_layernorm_fwd(x2.const_data_ptr(), ptr(w), ptr(b), y.data_ptr(), mean ? mean->data_ptr<float>() : nullptr,
-                       rstd ? rstd->data_ptr<float>() : nullptr, rows, D, x2.stride(0), D, dtype_code(x2.scalar_type()),
-                       weight_code(x2, w, b), (float)eps, cur_stream()),
+  run(mb_layernorm_fwd(x2.const_data_ptr(), ptr(w), ptr(b), y.data_ptr(), mean, mean ? mean + rows : nullptr, rows, D, x2.stride(0), D,
+                       dtype_code(x2.scalar_type()), weight_code(x2, w, b), (float)eps, cur_stream()),
       1, "layer_norm");
   return y;
 }
@@ -104,38 +104,35 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                             double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor weight = value(weight_in), bias = value(bias_in);
-    at::Tensor x2 = as_rows(x), mean, rstd;
+    at::Tensor x2 = as_rows(x), stats;
     at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
-    at::Tensor y = layer_norm_run(x2, w, b, x.sizes(), eps, &mean, &rstd);
-    ctx->save_for_backward({x2, w, mean, rstd});
-    ctx->saved_data["shape"] = x.sizes();
-    ctx->saved_data["w_dtype"] = (int64_t)weight_code(x, w, b);
-    ctx->saved_data["wants"] =
-        std::vector<bool>{x.requires_grad(), weight.defined() && weight.requires_grad(), bias.defined() && bias.requires_grad()};
+    at::Tensor y = layer_norm_run(x2, w, b, x.sizes(), eps, &stats);
+    ctx->save_for_backward({x2, w, stats});
+    ctx->saved_data["wants"] = (int64_t)(x.requires_grad() | (weight.defined() && weight.requires_grad()) << 1 |
+                                         (bias.defined() && bias.requires_grad()) << 2 | (weight_code(x, w, b) == MB_F32) << 3);
     return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("layer_norm");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x2 = saved[0], &w = saved[1], &mean = saved[2], &rstd = saved[3];
+    const at::Tensor &x2 = saved[0], &w = saved[1], &stats = saved[2];
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     c10::cuda::CUDAGuard guard(x2.device());
-    const int64_t rows = x2.size(0), D = x2.size(1);
-    const auto wants = ctx->saved_data["wants"].toBoolList();
-    const int w_code = (int)ctx->saved_data["w_dtype"].toInt();
+    const int64_t rows = x2.size(0), D = x2.size(1), wants = ctx->saved_data["wants"].toInt();
+    const int w_code = wants & 8 ? MB_F32 : dtype_code(x2.scalar_type());
     const auto w_options = x2.options().dtype(w_code == MB_F32 ? at::kFloat : x2.scalar_type());
     at::Tensor dy = as_rows(grads[0]), dx, dw, db, partial;
-    if (wants[0]) dx = at::empty(ctx->saved_data["shape"].toIntVector(), x2.options());
-    if (wants[1]) dw = rows ? at::empty({D}, w_options) : at::zeros({D}, w_options);
-    if (wants[2]) db = rows ? at::empty({D}, w_options) : at::zeros({D}, w_options);
-    if (rows && (wants[1] || wants[2]))
-      partial = at::empty({mb_layernorm_bwd_parts(rows, D), 2, D}, x2.options().dtype(at::kFloat));
-    run(mb_layernorm_bwd(x2.const_data_ptr(), ptr(w), dy.const_data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
-                         dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
-                         db.defined() ? db.data_ptr() : nullptr, partial.defined() ? partial.data_ptr<float>() : nullptr, rows,
-                         D, x2.stride(0), dy.stride(0), D, dtype_code(x2.scalar_type()), w_code, cur_stream()),
-        1 + (wants[1] || wants[2]), "layer_norm backward");
+    if (wants & 1) dx = at::empty(grads[0].sizes(), x2.options());
+    if (wants & 2) dw = rows ? at::empty({D}, w_options) : at::zeros({D}, w_options);
+    if (wants & 4) db = rows ? at::empty({D}, w_options) : at::zeros({D}, w_options);
+    if (rows && wants & 6) partial = at::empty({mb_layernorm_bwd_parts(rows, D), 2, D}, x2.options().dtype(at::kFloat));
+    const float* mean = stats.data_ptr<float>();
+    run(mb_layernorm_bwd(x2.const_data_ptr(), ptr(w), dy.const_data_ptr(), mean, mean + rows, dx.defined() ? dx.data_ptr() : nullptr,
+                         dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr,
+                         partial.defined() ? partial.data_ptr<float>() : nullptr, rows, D, x2.stride(0), dy.stride(0), D,
+                         dtype_code(x2.scalar_type()), w_code, cur_stream()),
+        rows ? 1 + (wants & 6 ? 1 : 0) : 0, "layer_norm backward");
     return {dx, dw, db, at::Tensor()};
   }
 };
@@ -146,8 +143,7 @@ at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTen
   c10::cuda::CUDAGuard guard(x.device());
   at::Tensor w = value(weight), b = value(bias);
   if (wants_grad(x) || wants_grad(w) || wants_grad(b)) return LayerNorm::apply(x, weight, bias, eps);
-  return layer_norm_run(as_rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, x.sizes(), eps, nullptr,
-                        nullptr);
+  return layer_norm_run(as_rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, x.sizes(), eps, nullptr);
 }
 
 // ---- rotary positions -----------------------------------------------------------------------------------------------------
@@ -456,14 +452,18 @@ at::Tensor as_tiles(const at::Tensor& t) {
 }
 int64_t pitch(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
-at::Tensor gated_run(const at::Tensor& x2, const at::Tensor& w2, at::IntArrayRef shape, int act, at::Tensor* gu) {
+// gu, scales: where the projections are kept for the backward pass, or null
+at::Tensor gated_run(const at::Tensor& x2, const at::Tensor& w2, at::IntArrayRef shape, int act, at::Tensor* gu, at::Tensor* scales) {
   const int64_t T = x2.size(0), K = x2.size(1), F = w2.size(0) / 2;
   at::Tensor h = at::empty(shape, x2.options());
-  if (gu) *gu = at::empty({T, 2 * F}, x2.options());
+  if (gu) {
+    *gu = at::empty({T, 2 * F}, x2.options().dtype(at::kHalf));
+    *scales = at::empty({T, 2 * (int64_t)mb_gated_scale_pitch((int)F)}, x2.options().dtype(at::kByte));
+  }
   const int dev = x2.get_device();
   check_kernel_status(dev);
-  run(mb_gated_fwd_bf16(x2.const_data_ptr(), w2.const_data_ptr(), h.data_ptr(), gu ? gu->data_ptr() : nullptr, T, (int)F, (int)K,
-                        pitch(x2), pitch(w2), F, 2 * F, act, kernel_status(dev), 0, cur_stream()),
+  run(mb_gated_fwd_bf16(x2.const_data_ptr(), w2.const_data_ptr(), h.data_ptr(), gu ? gu->data_ptr() : nullptr,
+                        gu ? scales->data_ptr() : nullptr, T, (int)F, (int)K, pitch(x2), pitch(w2), F, act, kernel_status(dev), 0, cur_stream()),
       1, "gated_linear");
   return h;
 }
@@ -477,12 +477,11 @@ std::vector<int64_t> gated_shape(const at::Tensor& x, const at::Tensor& w) {
 struct Gated : torch::autograd::Function<Gated> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t act) {
     at::AutoDispatchBelowADInplaceOrView below;
-    at::Tensor x2 = as_tiles(x), w2 = as_tiles(w), gu;
-    at::Tensor h = gated_run(x2, w2, gated_shape(x, w), (int)act, &gu);
-    ctx->save_for_backward({x2, w2, gu});
-    ctx->saved_data["shape"] = x.sizes();
+    at::Tensor x2 = as_tiles(x), w2 = as_tiles(w), gu, scales;
+    at::Tensor h = gated_run(x2, w2, gated_shape(x, w), (int)act, &gu, &scales);
+    ctx->save_for_backward({x2, w2, gu, scales});
     ctx->saved_data["act"] = act;
-    ctx->saved_data["wants"] = std::vector<bool>{x.requires_grad(), w.requires_grad()};
+    ctx->saved_data["wants"] = (int64_t)(x.requires_grad() | w.requires_grad() << 1);
     return h;
   }
 
@@ -490,18 +489,20 @@ struct Gated : torch::autograd::Function<Gated> {
     once("gated_linear");
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x2 = saved[0], &w2 = saved[1], &gu = saved[2];
+    const at::Tensor &x2 = saved[0], &w2 = saved[1], &gu = saved[2], &scales = saved[3];
     c10::cuda::CUDAGuard guard(x2.device());
     const int64_t T = x2.size(0), K = x2.size(1), F = w2.size(0) / 2;
-    const auto wants = ctx->saved_data["wants"].toBoolList();
+    const int64_t wants = ctx->saved_data["wants"].toInt();
+    std::vector<int64_t> shape = grads[0].sizes().vec();
+    shape.back() = K;
     at::Tensor dh = as_tiles(grads[0]), dgu = at::empty({T, 2 * F}, x2.options()), dx, dw;
-    if (wants[0]) dx = at::empty(ctx->saved_data["shape"].toIntVector(), x2.options());
-    if (wants[1]) dw = T ? at::empty({2 * F, K}, x2.options()) : at::zeros({2 * F, K}, x2.options());
+    if (wants & 1) dx = at::empty(shape, x2.options());
+    if (wants & 2) dw = T ? at::empty({2 * F, K}, x2.options()) : at::zeros({2 * F, K}, x2.options());
     if (T) {
       const int dev = x2.get_device();
       uint32_t* status = kernel_status(dev);
       check_kernel_status(dev);
-      run(mb_gated_bwd_bf16(gu.const_data_ptr(), dh.const_data_ptr(), dgu.data_ptr(), T, (int)F, 2 * F, pitch(dh), 2 * F,
+      run(mb_gated_bwd_bf16(gu.const_data_ptr(), scales.const_data_ptr(), dh.const_data_ptr(), dgu.data_ptr(), T, (int)F, pitch(dh),
                             (int)ctx->saved_data["act"].toInt(), cur_stream()),
           1, "gated_linear backward");
       // dx[T, K] = dgu[T, 2F] w[2F, K], dw[2F, K] = dgu^T x: the transposed operands are read as they lie
@@ -524,7 +525,7 @@ at::Tensor gated_linear(const at::Tensor& x, const at::Tensor& w, const std::str
   c10::cuda::CUDAGuard guard(x.device());
   const int act = act_code(activation);
   if (wants_grad(x) || wants_grad(w)) return Gated::apply(x, w, (int64_t)act);
-  return gated_run(as_tiles(x), as_tiles(w), gated_shape(x, w), act, nullptr);
+  return gated_run(as_tiles(x), as_tiles(w), gated_shape(x, w), act, nullptr, nullptr);
 }
 
 }  // namespace

@@ -111,29 +111,33 @@ static void rows_shape(int F, int K, int device, int& width, int& split) {
   width = ((F + ctas - 1) / ctas + 7) / 8 * 8;
 }
 
-// dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F], bound by their bytes.
-// The results are rounded to bf16 because the two matrix products that follow take bf16 operands.
+// dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F] and a byte per 16 of the kept
+// projections, bound by their bytes. The results are rounded to bf16 because the two matrix products that follow take bf16 operands.
+// A thread keeps its 8 columns and walks down the rows, so no index is divided.
 template <int kAct>
 __global__ void __launch_bounds__(256)
-    gated_bwd_kernel(const __nv_bfloat16* __restrict__ gu, const __nv_bfloat16* __restrict__ dh, __nv_bfloat16* __restrict__ dgu,
-                     int64_t T, int F, int64_t ldgu, int64_t lddh, int64_t lddgu) {
-  const int vecs = F / 8;
-  const int64_t total = T * vecs;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / vecs;
-    const int j = (int)(i % vecs) * 8;
+    gated_bwd_kernel(const __half* __restrict__ gu, const uint8_t* __restrict__ scales, int scale_pitch,
+                     const __nv_bfloat16* __restrict__ dh, __nv_bfloat16* __restrict__ dgu, int64_t T, int F, int64_t lddh) {
+  const int v = blockIdx.x * 256 + threadIdx.x, j = v * 8;
+  if (j >= F) return;
+#pragma unroll 2
+  for (int64_t t = blockIdx.y; t < T; t += gridDim.y) {
+    const __half* from = gu + t * 2 * F + j;
+    const uint8_t* e = scales + t * 2 * scale_pitch + v;
     float g[8], u[8], d[8];
-    load_vec<__nv_bfloat16, 8>(gu + t * ldgu + j, g);
-    load_vec<__nv_bfloat16, 8>(gu + t * ldgu + F + j, u);
+    load_vec<__half, 8>(from, g);
+    load_vec<__half, 8>(from + F, u);
     load_vec<__nv_bfloat16, 8>(dh + t * lddh + j, d);
+    const float sg = kept_scale(e[0]), su = kept_scale(e[scale_pitch]);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float2 a = activate_slope<kAct>(g[k]);
-      g[k] = d[k] * u[k] * a.y;
+      const float2 a = activate_slope<kAct>(g[k] * sg);
+      g[k] = d[k] * (u[k] * su) * a.y;
       u[k] = d[k] * a.x;
     }
-    store_vec<__nv_bfloat16, 8>(dgu + t * lddgu + j, g);
-    store_vec<__nv_bfloat16, 8>(dgu + t * lddgu + F + j, u);
+    __nv_bfloat16* to = dgu + t * 2 * F + j;
+    store_vec<__nv_bfloat16, 8>(to, g);
+    store_vec<__nv_bfloat16, 8>(to + F, u);
   }
 }
 
@@ -143,12 +147,14 @@ __global__ void __launch_bounds__(256)
 using namespace mb;
 using namespace mb::gated;
 
-extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, int64_t T, int F, int K, int64_t ldx, int64_t ldw,
-                                 int64_t ldh, int64_t ldgu, int act, uint32_t* status, uint64_t wait_ns, void* stream) {
+extern "C" int mb_gated_scale_pitch(int F) { return (F / 8 + 15) / 16 * 16; }
+
+extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, void* scales, int64_t T, int F, int K, int64_t ldx,
+                                 int64_t ldw, int64_t ldh, int act, uint32_t* status, uint64_t wait_ns, void* stream) {
   if (T <= 0) return MB_OK;
-  if (F <= 0 || K <= 0 || T > (1 << 30) || F > (1 << 29) || act < 0 || act > 2) return MB_ERR_ARG;
-  if (F % 8 || K % 8 || ldx % 8 || ldw % 8 || ldh % 8 || ldgu % 8) return MB_ERR_ALIGN;
-  if (!is_aligned(x, 16) || !is_aligned(w, 16) || !is_aligned(h, 16) || !is_aligned(gu, 16)) return MB_ERR_ALIGN;
+  if (F <= 0 || K <= 0 || T > (1 << 30) || F > (1 << 29) || act < 0 || act > 2 || !gu != !scales) return MB_ERR_ARG;
+  if (F % 8 || K % 8 || ldx % 8 || ldw % 8 || ldh % 8) return MB_ERR_ALIGN;
+  if (!is_aligned(x, 16) || !is_aligned(w, 16) || !is_aligned(h, 16) || !is_aligned(gu, 16) || !is_aligned(scales, 16)) return MB_ERR_ALIGN;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return MB_ERR_DRIVER;
   // Few rows: the weight's bytes bound the time and a 256-row tile would leave SMs idle (one token, F = 14336, K = 4096:
@@ -169,8 +175,9 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   p.K = K;
   p.h = (__nv_bfloat16*)h;
   p.ldh = ldh;
-  p.gu = (__nv_bfloat16*)gu;
-  p.ldgu = ldgu;
+  p.gu = (__half*)gu;
+  p.scales = (uint8_t*)scales;
+  p.scale_pitch = mb_gated_scale_pitch(F);
   p.tiles_m = (int)((T + kPairBM - 1) / kPairBM);
   p.tiles_n = (F + kHCols - 1) / kHCols;
   p.group_m = 4;
@@ -187,16 +194,16 @@ extern "C" int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu
   }
 }
 
-extern "C" int mb_gated_bwd_bf16(const void* gu, const void* dh, void* dgu, int64_t T, int F, int64_t ldgu, int64_t lddh,
-                                 int64_t lddgu, int act, void* stream) {
+extern "C" int mb_gated_bwd_bf16(const void* gu, const void* scales, const void* dh, void* dgu, int64_t T, int F, int64_t lddh, int act,
+                                 void* stream) {
   if (T <= 0) return MB_OK;
   if (F <= 0 || act < 0 || act > 2) return MB_ERR_ARG;
-  if (F % 8 || ldgu % 8 || lddh % 8 || lddgu % 8 || !is_aligned(gu, 16) || !is_aligned(dh, 16) || !is_aligned(dgu, 16))
-    return MB_ERR_ALIGN;
-  int64_t grid = (T * (F / 8) + 255) / 256;
-  if (grid > 148 * 16) grid = 148 * 16;
+  if (F % 8 || lddh % 8 || !is_aligned(gu, 16) || !is_aligned(dh, 16) || !is_aligned(dgu, 16)) return MB_ERR_ALIGN;
+  const int across = (F / 8 + 255) / 256;
+  const int64_t down = (148 * 16 + across - 1) / across;
+  const dim3 grid(across, (unsigned)(T < down ? T : down));
   auto k = act == kSilu ? gated_bwd_kernel<kSilu> : act == kGelu ? gated_bwd_kernel<kGelu> : gated_bwd_kernel<kGeluTanh>;
-  k<<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((const __nv_bfloat16*)gu, (const __nv_bfloat16*)dh, (__nv_bfloat16*)dgu, T, F,
-                                                   ldgu, lddh, lddgu);
+  k<<<grid, 256, 0, MB_STREAM(stream)>>>((const __half*)gu, (const uint8_t*)scales, mb_gated_scale_pitch(F),
+                                                   (const __nv_bfloat16*)dh, (__nv_bfloat16*)dgu, T, F, lddh);
   return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }

@@ -6,8 +6,9 @@
 // [0, 128) of the accumulator are gate columns, [128, 256) the up columns of the same h. The even CTA loads the gate rows of W
 // and the odd one the up rows, so each still brings 128 rows of x and 128 rows of W per 64-wide step, as in the plain
 // product, and a thread of the epilogue finds both factors of an h in its own TMEM lane. The activation runs on the fp32
-// accumulators: h is rounded once. With `gu` the two projections are written too (bf16, for the backward pass: 16 bits are
-// what the unfused layer keeps, and 32 would double the largest activation of a block).
+// accumulators: h is rounded once. For the backward pass the two projections are kept in 16 bits too (32 would double the
+// largest activation of a block): fp16 with one power of two per 8 columns, an eighth of bf16's rounding at 6 % more
+// bytes and the range of fp32. In bf16 they alone would add as much error to the gradients as all other roundings together.
 //
 // Bound by the tensor cores: 4 T F K flops. Against product + activation kernels it saves the write and read of [T, 2F]
 // (inference) or the read (training).
@@ -35,8 +36,10 @@ struct GatedParams {
   int T, F, K;
   __nv_bfloat16* h;
   int64_t ldh;
-  __nv_bfloat16* gu;  // [T, 2F] or null
-  int64_t ldgu;
+  // the kept projections, or null: fp16 mantissas [T, 2F] and scales [T, 2 scale_pitch], a byte per 8 columns (gate's, then up's)
+  __half* gu;
+  uint8_t* scales;
+  int scale_pitch;
   int tiles_m, tiles_n, group_m;
   int num_ctas;
   uint32_t* status;
@@ -54,7 +57,7 @@ __device__ __forceinline__ float activate(float g) {
 template <int kAct>
 __device__ __forceinline__ float2 activate_slope(float g) {
   if (kAct == kSilu) {
-    const float s = 1.f / (1.f + __expf(-g));
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
     return make_float2(g * s, s * (1.f + g * (1.f - s)));
   }
   if (kAct == kGelu) {
@@ -62,7 +65,7 @@ __device__ __forceinline__ float2 activate_slope(float g) {
     return make_float2(g * c, c + g * __expf(-0.5f * g * g) * 0.39894228f);
   }
   const float y2 = 1.5957691216f * (g + 0.044715f * g * g * g);
-  const float s = 1.f / (1.f + __expf(-y2));
+  const float s = __fdividef(1.f, 1.f + __expf(-y2));
   return make_float2(g * s, s + g * s * (1.f - s) * 1.5957691216f * (1.f + 0.134145f * g * g));
 }
 
@@ -81,6 +84,27 @@ __device__ __forceinline__ void gated_tile(const GatedParams& p, int t, int& tm,
   tn = r / gsz;
 }
 
+// 8 values v as fp16 mantissas of v / 2^(e - 127); returns e, which brings the largest finite one to 2^14 .. 2^15
+__device__ __forceinline__ uint32_t keep8(const float* v, uint4* to) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+    top = max(top, a < 0x7f800000u ? a : 0u);
+  }
+  const int e = max((int)(top >> 23) - 14, 1);
+  const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *to = make_uint4(w[0], w[1], w[2], w[3]);
+  return (uint32_t)e;
+}
+__device__ __forceinline__ float kept_scale(uint32_t e) { return __uint_as_float(e << 23); }
+
 // The epilogue's patch of shared memory per warp: 32 rows of three 64-byte pieces (32 columns of h, gate and up), padded so
 // that 16-byte accesses of eight rows meet no bank twice.
 constexpr int kPatchRow = 208;
@@ -96,7 +120,8 @@ __device__ __forceinline__ void patch_put(uint8_t* to, const float* v) {
                    pack_bf16x2(v[g * 8 + 4], v[g * 8 + 5]), pack_bf16x2(v[g * 8 + 6], v[g * 8 + 7]));
 }
 // one piece of the patch, 32 rows x 32 columns -> global memory, whole 64-byte runs
-__device__ __forceinline__ void patch_store(const uint8_t* piece, int lane, __nv_bfloat16* base, int64_t ld, int rows, int cols) {
+template <typename T>
+__device__ __forceinline__ void patch_store(const uint8_t* piece, int lane, T* base, int64_t ld, int rows, int cols) {
   const int col = (lane & 3) * 8;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -117,6 +142,7 @@ __device__ __forceinline__ void gated_epilogue(const GatedParams& p, uint32_t ta
   for (int c = 0; c < width; c += 32) {
     const int cols = min(p.F - (col0 + c), width - c);
     uint8_t* line = patch + lane * kPatchRow;
+    uint32_t eg = 0, eu = 0;
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       uint32_t rg[16], ru[16];
@@ -130,8 +156,12 @@ __device__ __forceinline__ void gated_epilogue(const GatedParams& p, uint32_t ta
         u[i] = __uint_as_float(ru[i]);
       }
       if (kSave) {
-        patch_put(line + 64 + half * 32, g);
-        patch_put(line + 128 + half * 32, u);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int shift = half * 16 + i * 8;
+          eg |= keep8(g + i * 8, reinterpret_cast<uint4*>(line + 64 + half * 32) + i) << shift;
+          eu |= keep8(u + i * 8, reinterpret_cast<uint4*>(line + 128 + half * 32) + i) << shift;
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) g[i] = activate<kAct>(g[i]) * u[i];
@@ -140,9 +170,15 @@ __device__ __forceinline__ void gated_epilogue(const GatedParams& p, uint32_t ta
     __syncwarp();
     patch_store(patch, lane, p.h + (int64_t)row0 * p.ldh + col0 + c, p.ldh, rows, cols);
     if (kSave) {
-      __nv_bfloat16* to = p.gu + (int64_t)row0 * p.ldgu + col0 + c;
-      patch_store(patch + 64, lane, to, p.ldgu, rows, cols);
-      patch_store(patch + 128, lane, to + p.F, p.ldgu, rows, cols);
+      __half* to = p.gu + (int64_t)row0 * 2 * p.F + col0 + c;
+      patch_store(patch + 64, lane, to, 2 * (int64_t)p.F, rows, cols);
+      patch_store(patch + 128, lane, to + p.F, 2 * (int64_t)p.F, rows, cols);
+      if (lane < rows && cols > 0) {
+        // (col0 + c is a multiple of 32 and the pitch one of 16: whole words, the last of which may reach into the padding)
+        uint8_t* e = p.scales + (int64_t)(row0 + lane) * 2 * p.scale_pitch + (col0 + c) / 8;
+        *reinterpret_cast<uint32_t*>(e) = eg;
+        *reinterpret_cast<uint32_t*>(e + p.scale_pitch) = eu;
+      }
     }
     __syncwarp();
   }
@@ -477,8 +513,10 @@ __device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width,
         }
       }
       if (kSave) {
-        store_vec<__nv_bfloat16, 8>(p.gu + t * p.ldgu + col, g);
-        store_vec<__nv_bfloat16, 8>(p.gu + t * p.ldgu + p.F + col, u);
+        __half* to = p.gu + (int64_t)t * 2 * p.F + col;
+        uint8_t* e = p.scales + (int64_t)t * 2 * p.scale_pitch + col / 8;
+        e[0] = (uint8_t)keep8(g, reinterpret_cast<uint4*>(to));
+        e[p.scale_pitch] = (uint8_t)keep8(u, reinterpret_cast<uint4*>(to + p.F));
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) g[k] = activate<kAct>(g[k]) * u[k];

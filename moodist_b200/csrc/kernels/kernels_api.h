@@ -267,13 +267,14 @@ int mb_distill_fwd(const mb_distill_t* d, void* grad, int64_t grad_stride, void*
 int mb_distill_bwd(const mb_distill_t* d, const float* gout, void* grad, int64_t grad_stride, void* stream);
 // x[0 .. n) *= s[0], in place; leaves x alone when s[0] is 1 (x: dtype, 16-byte aligned)
 int mb_scale_by(void* x, int64_t n, int dtype, const float* s, void* stream);
-// Gated projection (gated_gemm.cu): h[T, F] = act(x Wg^T) * (x Wu^T) for bf16 x[T, K] and w[2F, K] (gate rows first); gu
-// (may be null) receives the two projections [T, 2F]. act: 0 SiLU, 1 GELU, 2 GELU with tanh. F, K and the pitches are
-// multiples of 8, all addresses 16-byte aligned. The backward call turns dh and gu into dgu[T, 2F], the gradient of x w^T.
-int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, int64_t T, int F, int K, int64_t ldx, int64_t ldw,
-                      int64_t ldh, int64_t ldgu, int act, uint32_t* status, uint64_t wait_ns, void* stream);
-int mb_gated_bwd_bf16(const void* gu, const void* dh, void* dgu, int64_t T, int F, int64_t ldgu, int64_t lddh, int64_t lddgu,
-                      int act, void* stream);
+// Gated projection (gated_gemm.cu): h[T, F] = act(x Wg^T) * (x Wu^T) for bf16 x[T, K] and w[2F, K] (gate rows first). gu and
+// scales (both null when no backward pass follows) keep the two projections for it: fp16 [T, 2F] and bytes
+// [T, 2 mb_gated_scale_pitch(F)]. act: 0 SiLU, 1 GELU, 2 GELU with tanh. F, K and the pitches are multiples of 8, all addresses
+// 16-byte aligned. The backward call turns them and dh into bf16 dgu[T, 2F], the gradient of x w^T.
+int mb_gated_scale_pitch(int F);
+int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, void* scales, int64_t T, int F, int K, int64_t ldx, int64_t ldw,
+                      int64_t ldh, int act, uint32_t* status, uint64_t wait_ns, void* stream);
+int mb_gated_bwd_bf16(const void* gu, const void* scales, const void* dh, void* dgu, int64_t T, int F, int64_t lddh, int act, void* stream);
 
 #ifdef __cplusplus
 }

@@ -88,7 +88,8 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, activation: str = "silu") -> 
 
     bf16, ``F`` and ``K`` multiples of 8, any number of rows; ``activation`` is ``"silu"``, ``"gelu"`` or ``"gelu_tanh"``.
     The result is rounded once from fp32.  Differentiable (once) in both arguments: the forward pass then keeps the two
-    projections in bf16 and the backward pass is one elementwise kernel and two matrix products.
+    projections in 16 bits (fp16 with a power of two per 8 columns, so nothing overflows) and the backward pass is one elementwise
+    kernel, whose result is rounded to bf16, and two matrix products.
     """
     if x.is_cuda:
         return _C.gated_linear(x, w, activation)
