@@ -102,7 +102,6 @@ at::Tensor layer_norm_run(const at::Tensor& x2, const at::Tensor& w, const at::T
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& weight_in, const OptTensor& bias_in,
                             double eps) {
-    at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor weight = value(weight_in), bias = value(bias_in);
     at::Tensor x2 = as_rows(x), stats;
     at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
@@ -227,7 +226,6 @@ void rotary_run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qo, 
 struct Rotary : torch::autograd::Function<Rotary> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k_in, const at::Tensor& cos,
                                const at::Tensor& sin, const OptTensor& positions_in, bool interleaved) {
-    at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor k = value(k_in), positions = value(positions_in);
     at::Tensor qo = at::empty(q.sizes(), q.options()), ko = k.defined() ? at::empty(k.sizes(), k.options()) : at::Tensor();
     rotary_run(dense_last(q), dense_last(k), qo, ko, cos, sin, positions, interleaved, false, false);
@@ -309,7 +307,8 @@ void distill_check(const at::Tensor& logits, const at::Tensor& ids, const at::Te
               top.scalar_type());
   TORCH_CHECK(!top.requires_grad(), "moodist distill_loss: the teacher has no gradient (detach its logits)");
   TORCH_CHECK(ids.device() == logits.device() && top.device() == logits.device(), "moodist distill_loss: tensors on one device required");
-  TORCH_CHECK(tau > 0 && std::isfinite(tau), "moodist distill_loss: temperature must be positive");
+  TORCH_CHECK((float)tau > 0 && std::isfinite((float)tau) && std::isfinite(1 / (float)tau),
+              "moodist distill_loss: temperature must be positive, and it and its inverse finite in fp32");
   TORCH_CHECK(hard >= 0 && hard <= 1, "moodist distill_loss: hard_weight must be in [0, 1]");
   TORCH_CHECK(hard == 0 || targets.has_value(), "moodist distill_loss: hard_weight needs targets");
   if (targets.has_value()) {
@@ -353,7 +352,6 @@ mb_distill_t distill_args(const at::Tensor& z, const at::Tensor& ids, const at::
 struct Distill : torch::autograd::Function<Distill> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids_in, const at::Tensor& top_in,
                             const OptTensor& targets_opt, double tau, double hard, int64_t ignore_index, bool mean, double scale) {
-    at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor targets_in = value(targets_opt);
     const int64_t rows = logits.numel() / logits.size(-1), K = ids_in.size(-1);
     if (!rows) {
@@ -476,7 +474,6 @@ std::vector<int64_t> gated_shape(const at::Tensor& x, const at::Tensor& w) {
 
 struct Gated : torch::autograd::Function<Gated> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t act) {
-    at::AutoDispatchBelowADInplaceOrView below;
     at::Tensor x2 = as_tiles(x), w2 = as_tiles(w), gu, scales;
     at::Tensor h = gated_run(x2, w2, gated_shape(x, w), (int)act, &gu, &scales);
     ctx->save_for_backward({x2, w2, gu, scales});

@@ -784,7 +784,6 @@ extern "C" int mb_scale_by(void* x, int64_t n, int dtype, const float* s, void* 
   grid = grid < 1 ? 1 : grid > kSms * 8 ? kSms * 8 : grid;
   switch (dtype) {
     case MB_BF16: scale_by_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((__nv_bfloat16*)x, n, s); break;
-    case MB_F16: scale_by_kernel<__half><<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((__half*)x, n, s); break;
     case MB_F32: scale_by_kernel<float><<<(unsigned)grid, 256, 0, MB_STREAM(stream)>>>((float*)x, n, s); break;
     default: return MB_ERR_ARG;
   }

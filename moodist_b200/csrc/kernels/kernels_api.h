@@ -265,7 +265,7 @@ typedef struct {
 int mb_distill_fwd(const mb_distill_t* d, void* grad, int64_t grad_stride, void* stream);
 // grad[rows, V] = d loss / d logits * gout[0], from the scratch and stats that a forward call without grad left.
 int mb_distill_bwd(const mb_distill_t* d, const float* gout, void* grad, int64_t grad_stride, void* stream);
-// x[0 .. n) *= s[0], in place; leaves x alone when s[0] is 1 (x: dtype, 16-byte aligned)
+// x[0 .. n) *= s[0], in place; leaves x alone when s[0] is 1 (x: MB_BF16 or MB_F32, 16-byte aligned)
 int mb_scale_by(void* x, int64_t n, int dtype, const float* s, void* stream);
 // Gated projection (gated_gemm.cu): h[T, F] = act(x Wg^T) * (x Wu^T) for bf16 x[T, K] and w[2F, K] (gate rows first). gu and
 // scales (both null when no backward pass follows) keep the two projections for it: fp16 [T, 2F] and bytes

@@ -28,10 +28,11 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
   return __float2half_rn(v);
 }
 
-// N elements as they lie in memory: 32-bit words (a struct of 16-bit members is taken apart and put together again member by
-// member in registers), or the single 16-bit element.
+// N elements as they lie in memory, in 32-bit words (a struct of 16-bit members is taken apart and put together again member by
+// member in registers) or, alone, a 16-bit element. On a 16-byte boundary at most: eight fp32 weights beside eight 16-bit
+// elements are two loads.
 template <typename T, int N, bool kWords = sizeof(T) * N % 4 == 0>
-struct alignas(sizeof(T) * N) Pack {
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   uint32_t w[sizeof(T) * N / 4];
 };
 template <typename T, int N>
@@ -177,17 +178,6 @@ __device__ __forceinline__ float block_reduce_sum(float v, float* red) {
   __syncthreads();
   return warp_reduce_sum(lane < kThreads / 32 ? red[lane] : 0.f);
 }
-template <int kThreads>
-__device__ __forceinline__ float block_reduce_max(float v, float* red) {
-  v = warp_reduce_max(v);
-  if (kThreads == 32) return v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  return warp_reduce_max(lane < kThreads / 32 ? red[lane] : -INFINITY);
-}
-
 inline bool is_aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 }  // namespace mb

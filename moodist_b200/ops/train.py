@@ -342,6 +342,10 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     Logits are bf16, fp16 or fp32, ids int64 or int32, teacher logits bf16, fp16 or fp32, targets int64.  Differentiable
     (once) in ``logits``, which stay as they are: where :func:`cross_entropy` is wanted as well, take it in here through
     ``targets``, since its own backward pass overwrites the logits that this one reads.
+
+    On CUDA the forward pass makes the gradient of bf16 and fp32 logits as well (when they require one), so that they are
+    read once: call it under ``torch.no_grad()`` where only the loss is wanted.  The backward pass then hands that gradient
+    out, once per forward pass, and only touches it if the loss was scaled afterwards (``scale`` costs nothing).
     """
     if reduction not in ("mean", "sum"):
         raise ValueError(f"moodist distill_loss: reduction must be 'mean' or 'sum', not {reduction!r}")

@@ -84,6 +84,55 @@ def test_layer_norm_partial_gradients_and_refusals():
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_layer_norm_wide_weights_on_16_byte_boundaries(dtype):
+    """fp32 weights that start 16 but not 32 bytes from a boundary, beside 16-bit rows that are read in vectors."""
+    from moodist_b200.ops.train import layer_norm
+
+    torch.manual_seed(8)
+    for D in (64, 1024, 4096, 16384):
+        x, dy = _randn(20, D, dtype=dtype), _randn(20, D, dtype=dtype)
+        w, b = (_randn(D + 4)[4:].requires_grad_() for _ in range(2))
+        x.requires_grad_()
+        y = layer_norm(x, w, b)
+        want = oracle.layer_norm(x, w, b, 1e-5, dy)
+        oracle.assert_within(y, *want["y"], "y")
+        for got, name in zip(torch.autograd.grad(y, (x, w, b), dy), ("dx", "dw", "db")):
+            oracle.assert_within(got, *want[name], name)
+
+
+def test_changes_between_forward_and_backward_are_noticed():
+    """What the backward pass reads must not have been written since, views of it included."""
+    from moodist_b200.ops.gemm import gated_linear
+    from moodist_b200.ops.train import distill_loss, layer_norm, rotary, rotary_tables
+
+    def changed(make, touch):
+        out = make()
+        with torch.no_grad():
+            touch.add_(1)
+        with pytest.raises(RuntimeError, match="inplace"):
+            out.sum().backward()
+
+    x3, w = _randn(2, 3, 16), _randn(16).requires_grad_()
+    changed(lambda: layer_norm(x3, w), x3)
+    changed(lambda: layer_norm(x3, w), w)
+    x, wg = _randn(2, 3, 16, dtype=torch.bfloat16).requires_grad_(), _randn(32, 16, dtype=torch.bfloat16).requires_grad_()
+    changed(lambda: gated_linear(x, wg), x)
+    changed(lambda: gated_linear(x, wg), wg)
+    cos, sin = rotary_tables(8, 4, device="cuda")
+    changed(lambda: rotary(x3.view(2, 3, 2, 8).requires_grad_(), None, cos, sin)[0], cos)
+    z = _randn(2, 3, 16, dtype=torch.float16).requires_grad_()
+    ids, top = torch.zeros(2, 3, 2, device="cuda", dtype=torch.long), _randn(2, 3, 2)
+    changed(lambda: distill_loss(z, ids, top), z)
+    # bf16 logits are done with once the loss is there
+    z = _randn(2, 3, 16, dtype=torch.bfloat16).requires_grad_()
+    want = torch.autograd.grad(distill_loss(z, ids, top), z)[0]
+    loss = distill_loss(z, ids, top)
+    with torch.no_grad():
+        z.zero_()
+    assert torch.equal(torch.autograd.grad(loss, z)[0], want)
+
+
 # ---- rotary positions ---------------------------------------------------------------------------------------------
 
 
@@ -202,6 +251,16 @@ def test_distill_refusals_and_repeated_backward():
     before = z.detach().clone()
     torch.autograd.grad(distill_loss(z, ids, top, targets), z)
     assert torch.equal(z.detach().nan_to_num(1.0), before.nan_to_num(1.0))  # the logits stay
+    # one backward pass per forward pass, fp16 apart, whose gradient is not made beforehand
+    for dtype in DTYPES:
+        x = before.to(dtype).requires_grad_()
+        loss = distill_loss(x, ids, top, targets)
+        torch.autograd.grad(loss, x, retain_graph=True)
+        if dtype == torch.float16:
+            torch.autograd.grad(loss, x)
+        else:
+            with pytest.raises(RuntimeError, match="taken already"):
+                torch.autograd.grad(loss, x)
 
 
 # ---- gated projection ---------------------------------------------------------------------------------------------
