@@ -217,6 +217,25 @@ def test_distill_loss(rows, V, K, dtype):
         z = z.detach()
 
 
+@pytest.mark.parametrize("rows,V,K,dtype", [(400, 9001, 3, torch.bfloat16), (310, 8200, 5, torch.float16), (40, 20000, 1100, torch.float32),
+                                            (3000, 72, 9, torch.bfloat16), (150, 40000, 2, torch.float32)])
+def test_distill_many_rows(rows, V, K, dtype):
+    """More rows than CTAs, rows that do not count among them, entries beyond what is compared in shared memory."""
+    from moodist_b200.ops.train import distill_loss
+
+    z, ids, top, targets = distill_case(rows, V, K, dtype, "cuda", seed=rows)
+    out = torch.rand(rows, device="cuda") < 0.3
+    ids[out & (torch.arange(rows, device="cuda") % 2 == 0)] = V + 1
+    targets[out & (torch.arange(rows, device="cuda") % 2 == 1)] = -100
+    z.requires_grad_()
+    for tau, hard, reduction in ((2.0, 0.5, "mean"), (1.0, 0.0, "sum")):
+        loss = distill_loss(z, ids, top, targets, temperature=tau, hard_weight=hard, reduction=reduction)
+        want = oracle.distill(z, ids, top, targets, tau, hard, reduction)
+        oracle.assert_within(loss, *want["loss"], "loss")
+        (dz,) = torch.autograd.grad(loss, z)
+        oracle.assert_within(dz, *want["dz"], "dz")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_distill_layouts_types_and_incoming_gradient(dtype):
     from moodist_b200.ops.train import distill_loss
@@ -268,7 +287,7 @@ def test_distill_refusals_and_repeated_backward():
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("T,F,K", [(1, 8, 8), (0, 16, 16), (3, 200, 72), (17, 1000, 1016), (127, 136, 64), (128, 128, 512), (129, 264, 256), (301, 328, 200),
-                                   (1000, 520, 264)])
+                                   (1000, 520, 264), (5, 264, 4096), (128, 1000, 1024), (100, 1184, 2056), (33, 10008, 256), (3, 19000, 136)])
 def test_gated_linear(T, F, K, act):
     from moodist_b200.ops.gemm import gated_linear
 
@@ -309,6 +328,42 @@ def test_gated_linear_layouts_and_refusals():
         torch.autograd.grad(gated_linear(x_, w_).sum(), x_, create_graph=True)
     with pytest.raises(RuntimeError, match="device"):
         gated_linear(x_, w_.cpu())
+
+
+# ---- more than 2^31 elements ----------------------------------------------------------------------------------------
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of tensors of more than 2^31 elements, against the same rows on their own."""
+    from moodist_b200.ops.train import distill_loss, layer_norm, rotary, rotary_tables
+
+    def big(*shape):
+        return torch.empty(*shape, device="cuda", dtype=torch.bfloat16).normal_()
+
+    x = big(140000, 16384)
+    w = _randn(16384, dtype=torch.bfloat16)
+    dy = x[-1:].expand(140000, 16384)
+    x.requires_grad_()
+    y = layer_norm(x, w)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    last = x.detach()[-3:].clone().requires_grad_()
+    y3 = layer_norm(last, w)
+    assert torch.equal(y[-3:], y3) and torch.equal(dx[-3:], torch.autograd.grad(y3, last, dy[-3:])[0])
+    del x, y, dx, dy
+
+    q = big(2, 150000, 64, 128)
+    cos, sin = rotary_tables(128, 150000, device="cuda")
+    a, _ = rotary(q, None, cos, sin)
+    at = torch.arange(149997, 150000, device="cuda")
+    assert torch.equal(a[1:, -3:], rotary(q[1:, -3:], None, cos, sin, at)[0])
+    del q, a
+
+    z = big(17000, 128256).requires_grad_()
+    ids, top = torch.randint(0, 128256, (17000, 4), device="cuda"), _randn(17000, 4)
+    (dz,) = torch.autograd.grad(distill_loss(z, ids, top, reduction="sum"), z)
+    last = z.detach()[-160:].clone().requires_grad_()
+    (d3,) = torch.autograd.grad(distill_loss(last, ids[-160:], top[-160:], reduction="sum"), last)
+    assert torch.equal(dz[-160:], d3)
 
 
 # ---- together -----------------------------------------------------------------------------------------------------
