@@ -6,7 +6,8 @@
 //
 // Bound by the bytes of q and k, read once and written once. A thread takes V pairs of one token (V * sizeof(T) = 16 bytes where
 // sizes, strides and addresses allow: two vector loads and two vector stores) in four neighbouring heads: eight loads in
-// flight, and the cosines and sines, which are twice the bytes of the pairs of one 16-bit head, are read once for the four.
+// flight, and the cosines and sines, which are twice the bytes of the pairs of one 16-bit head, are read once for the four
+// (two heads per thread: 35 us where four take 31). 8192 tokens, 40 heads of 128, bf16: 31 us, 5.5 TB/s, each way.
 #include "kernels_api.h"
 #include "vec_io.cuh"
 
