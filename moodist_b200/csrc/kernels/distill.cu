@@ -464,13 +464,13 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 // What is left of a row when its walk is over: its named places and its loss wait for the next barrier, which is that of the
-// row after.
+// row after. In shared memory, with the threads' teacher entries: in registers it would be spilled inside the walks.
 template <bool kTwo>
 struct Unfinished {
-  int64_t r = -1;
+  int64_t r;
   Slope<kTwo> slope;
-  int id, live;
-  float p, z, st, s1;
+  int live;
+  float st, s1;
 };
 
 // kTwo: the two terms need different exponentials (a hard term, and tau is not 1). The grid is clusters of `parts` CTAs, one row
@@ -481,6 +481,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   constexpr int kV = Row<T>::kV, kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float red[2][4][kWarps];  // by row parity: a peer may still read the row before's
+  __shared__ Unfinished<kTwo> left[2];  // by row parity too
+  __shared__ float kept_p[kThreads], kept_z[kThreads];
+  __shared__ int kept_id[kThreads];
   __shared__ int shared_count;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float inv_tau = 1.f / d.tau;
@@ -492,13 +495,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   In stream;
   stream.begin(ring, d, part, grad != nullptr);
   int parity = 0;
-  Unfinished<kTwo> u;
+  bool any = false;
   auto finish = [&](int from) {
+    const Unfinished<kTwo> u = left[from];
     const T* z = reinterpret_cast<const T*>(d.logits) + u.r * d.stride;
     const int64_t t = d.hard > 0.f ? d.targets[u.r] : -1;
     if (grad) {
       T* g = grad + u.r * grad_stride;
-      named_place<T, kThreads, kTwo>(d, u.r, g, part, u.slope, a_soft, a_hard, t, u.id, u.p, u.z);
+      named_place<T, kThreads, kTwo>(d, u.r, g, part, u.slope, a_soft, a_hard, t, kept_id[threadIdx.x], kept_p[threadIdx.x], kept_z[threadIdx.x]);
       if (d.K > kThreads || (t >= 0 && u.live == 1)) other_places<T, kThreads, kTwo>(d, u.r, z, g, part, u.slope, a_soft, a_hard, t, u.live);
     }
     if (warp == 0 && part.rank == 0) {
@@ -534,8 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     const float my_p = next_p;
     float my_z = 0.f;
     if (live && my_p != 0.f) my_z = to_f32(z[my_id]);
-    peek(r + part.step());
     if (!live) {
+      peek(r + part.step());
       if (threadIdx.x == 0 && part.rank == 0) d.row_loss[r] = 0.f;
       if (grad) row_zeros<T, kThreads>(g + part.from, part.count);
       continue;
@@ -593,15 +597,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       st = warp_reduce_sum(wt * exp2_fast((wm - m) * run.c));
       s1 = kTwo ? warp_reduce_sum(w1 * exp2_fast((wm - m) * kLog2e)) : st;
     }
-    if (u.r >= 0) finish(parity ^ 1);
-    u.r = r;
-    u.slope = Slope<kTwo>{m, run.c, kTwo ? a_soft / st : (a_soft + a_hard) / st, a_hard / s1};
-    u.id = my_id;
-    u.live = live;
-    u.p = my_p;
-    u.z = my_z;
-    u.st = st;
-    u.s1 = s1;
+    if (any) finish(parity ^ 1);
+    any = true;
+    const Slope<kTwo> slope{m, run.c, kTwo ? a_soft / st : (a_soft + a_hard) / st, a_hard / s1};
+    kept_id[threadIdx.x] = my_id;
+    kept_p[threadIdx.x] = my_p;
+    kept_z[threadIdx.x] = my_z;
+    if (threadIdx.x == 0) left[parity] = Unfinished<kTwo>{r, slope, live, st, s1};
     if (part.rank == 0) {
       // the teacher's entries against q, but for log(st)
       float ce = my_p != 0.f ? my_p * (my_z - m) * inv_tau : 0.f;
@@ -612,11 +614,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       ce = warp_reduce_sum(ce);
       if (lane == 0) red[parity][3][warp] = ce;
     }
-    if (grad) row_gradient<T, kThreads, kTwo>(row, z + part.from, g + part.from, stream, u.slope);
+    peek(r + part.step());
+    if (grad) row_gradient<T, kThreads, kTwo>(row, z + part.from, g + part.from, stream, slope);
     parity ^= 1;
   }
   __syncthreads();
-  if (u.r >= 0) finish(parity ^ 1);
+  if (any) finish(parity ^ 1);
   if (parts > 1) cluster_barrier();  // the peers no longer read this CTA's sums
   // the last CTA to get here adds the row losses up, in a fixed order
   __shared__ bool last;
