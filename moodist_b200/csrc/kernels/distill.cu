@@ -7,10 +7,11 @@
 // Bound by the bytes of the logits, read once, and of the gradient, written once. The gradient's scale is known in the forward
 // pass up to the incoming scalar (which is 1 unless the loss is scaled afterwards), so the forward pass writes it: a CTA walks a
 // row twice, first from memory for the maximum and the sum of exponentials, then for the gradient from L2, where the rows in
-// work (148 of 256 KB at 128256 words, one CTA of 1024 threads per SM) stay. 4096 x 128256 bf16: 458 us, 4.6 TB/s, held back by
-// the exponentials' unit (half of the time busy) and the instructions around it (56 % of the issue slots). Two CTAs per SM
-// with a row each read 1.4 times the logits from memory (520 us), and two that share rows as a cluster pay for their barriers
-// (474 us). Where there are fewer rows than SMs, clusters do share them.
+// work (148 of 256 KB at 128256 words, one CTA of 1024 threads per SM) stay. 4096 x 128256 bf16: 440 us, 4.8 TB/s, held back by
+// the exponentials' unit (half of the time busy) and the instructions around it (56 % of the issue slots; every fourth
+// exponential as a polynomial on the multiply-add units took 530 us). Two CTAs per SM with a row each read 1.4 times the logits
+// from memory, and two that share rows as a cluster pay for their barriers (520 and 474 us when one CTA took 458). Where there
+// are fewer rows than SMs, clusters do share them.
 // fp16 is the exception: its gradients would underflow before a loss scale reaches them, so there the backward pass reads the
 // logits again.
 // Sums and row statistics are fp32; sums have a fixed order, so the same inputs give the same bits.
