@@ -504,8 +504,8 @@ struct Gated : torch::autograd::Function<Gated> {
           1, "gated_linear backward");
       // dx[T, K] = dgu[T, 2F] w[2F, K], dw[2F, K] = dgu^T x: the transposed operands are read as they lie
       if (dx.defined())
-        run(mb_gemm_bf16(dgu.const_data_ptr(), w2.const_data_ptr(), dx.data_ptr(), (int)T, (int)K, (int)(2 * F), 2 * F, pitch(w2), K, 0, 1,
-                         0, 0, status, 0, cur_stream()),
+        run(mb_gated_dx_bf16(dgu.const_data_ptr(), w2.const_data_ptr(), dx.data_ptr(), T, (int)F, (int)K, 2 * F, pitch(w2), K, status, 0,
+                             cur_stream()),
             1, "gated_linear backward");
       if (dw.defined())
         run(mb_gemm_bf16(dgu.const_data_ptr(), x2.const_data_ptr(), dw.data_ptr(), (int)(2 * F), (int)K, (int)T, 2 * F, pitch(x2), K, 1, 1,

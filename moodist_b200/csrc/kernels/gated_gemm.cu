@@ -90,25 +90,64 @@ static int launch_rows(const GatedParams& p, int width, int n, int split, const 
   return cudaLaunchKernelEx(&cfg, kern, p, width, n, split, tx, tw) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
-// Columns of h per CTA and CTAs per K range of the few-rows kernel. One wave of CTAs is to cover F with the narrowest width
-// (a multiple of 8) that does; from 128 SMs' worth of columns up it takes more waves. Where F is so small that tiles of 64
-// columns leave SMs over, up to 8 CTAs split K, as long as each keeps 8 steps of 64 (F = 1184, K = 4096: 8.5 us in four parts,
-// 24 us in one). Clusters of several CTAs do not fill every SM, so a sixteenth of them is not counted on then.
-static void rows_shape(int F, int K, int device, int& width, int& split) {
+static int device_sms(int device) {
   static int sms[kMaxDevices];
   if (sms[device] == 0) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
     sms[device] = n;
   }
+  return sms[device];
+}
+
+// How many clusters of `split` CTAs, one per SM, run at once: the SMs are not a multiple of a cluster in every part of the GPU.
+// Asked once per device, for splits of 1, 2, 4 and 8.
+template <auto kKernel>
+static int active_clusters(int split, int device) {
+  static int known[kMaxDevices][4];
+  int& n = known[device][split >= 8 ? 3 : split / 2];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(device_sms(device) / split * split, 1, 1);
+    cfg.blockDim = dim3(kNumThreads, 1, 1);
+    cfg.dynamicSmemBytes = kRowsSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&got, kKernel, &cfg) != cudaSuccess || got <= 0) {
+      cudaGetLastError();
+      got = device_sms(device) * 3 / 4 / split;
+    }
+    n = got;
+  }
+  return n;
+}
+
+// Columns of h per CTA and CTAs per K range of the few-rows kernel. One wave of CTAs is to cover F with the narrowest width
+// (a multiple of 8) that does; from 128 SMs' worth of columns up it takes more waves. Where F is so small that tiles of 64
+// columns leave SMs over, up to 8 CTAs split K, as long as each keeps 8 steps of 64 (F = 1184, K = 4096: 8.5 us in four parts,
+// 24 us in one).
+static void rows_shape(int F, int K, int device, int& width, int& split) {
+  const int sms = device_sms(device);
   for (split = 8; split > 1; split /= 2) {
-    const int tiles = (sms[device] - sms[device] / 16) / split;
+    const int tiles = active_clusters<gated_rows_kernel<kSilu, false>>(split, device);
     width = ((F + tiles - 1) / tiles + 7) / 8 * 8;
     if (width <= 64 && K >= split * 8 * BK) return;
   }
-  const int waves = (F + 128 * sms[device] - 1) / (128 * sms[device]);
-  const int ctas = waves * sms[device];
+  const int waves = (F + 128 * sms - 1) / (128 * sms);
+  const int ctas = waves * sms;
   width = ((F + ctas - 1) / ctas + 7) / 8 * 8;
+}
+
+__global__ void __launch_bounds__(kNumThreads, 1)
+    gated_dx_kernel(const __grid_constant__ DxParams p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_d) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  gated_dx_body(p, &tmap_w, &tmap_d, smem_raw);
 }
 
 // dgu[:, :F] = dh * u * act'(g), dgu[:, F:] = dh * act(g): three reads and two writes of [T, F] and a byte per 16 of the kept
@@ -206,4 +245,57 @@ extern "C" int mb_gated_bwd_bf16(const void* gu, const void* scales, const void*
   k<<<grid, 256, 0, MB_STREAM(stream)>>>((const __half*)gu, (const uint8_t*)scales, mb_gated_scale_pitch(F),
                                                    (const __nv_bfloat16*)dh, (__nv_bfloat16*)dgu, T, F, lddh);
   return cudaPeekAtLastError() == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+}
+
+extern "C" int mb_gated_dx_bf16(const void* dgu, const void* w, void* dx, int64_t T, int F, int K, int64_t lddgu, int64_t ldw,
+                                int64_t lddx, uint32_t* status, uint64_t wait_ns, void* stream) {
+  if (T <= 0) return MB_OK;
+  if (F <= 0 || K <= 0 || T > (1 << 30) || F > (1 << 29)) return MB_ERR_ARG;
+  if (F % 8 || K % 8 || lddgu % 8 || ldw % 8 || lddx % 8 || !is_aligned(dgu, 16) || !is_aligned(w, 16) || !is_aligned(dx, 16))
+    return MB_ERR_ALIGN;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return MB_ERR_DRIVER;
+  const int sms = device_sms(device);
+  // Up to a quarter of the SMs' worth of 256 x 256 tiles the split kernel is ahead (us, split and tiles): 1 row, 14336 -> 4096
+  // 38 and 161; 256, 11008 -> 4096 51 and 106; 1024, 1408 -> 2048 18 and 20, which is where it ends.
+  const int64_t pair_tiles = (T + kPairBM - 1) / kPairBM * ((K + BN - 1) / BN);
+  if (pair_tiles * 4 > sms)
+    return mb_gemm_bf16(dgu, w, dx, (int)T, K, 2 * F, lddgu, ldw, lddx, 0, 1, 0, 0, status, wait_ns, stream);
+  DxParams p{};
+  p.T = (int)T;
+  p.K = K;
+  p.R = 2 * F;
+  p.dx = (__nv_bfloat16*)dx;
+  p.lddx = lddx;
+  const int row_tiles = (int)((T + 255) / 256);
+  p.n = (int)((T + row_tiles - 1) / row_tiles + 15) / 16 * 16;
+  const int tiles = (K + BM - 1) / BM;
+  p.split = 8;
+  while (p.split > 1 && (tiles * row_tiles > active_clusters<gated_dx_kernel>(p.split, device) || p.R < p.split * 4 * BK)) p.split /= 2;
+  p.status = status;
+  p.wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
+  CUtensorMap tw, td;
+  int rc = gemm::make_tmap_bf16(&tw, w, 2 * (uint64_t)F, K, ldw, BK);
+  if (rc) return rc;
+  rc = gemm::make_tmap_bf16(&td, dgu, T, 2 * (uint64_t)F, lddgu, p.n);
+  if (rc) return rc;
+  static bool configured[kMaxDevices];
+  if (!configured[device]) {
+    if (cudaFuncSetAttribute(gated_dx_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) != cudaSuccess) return MB_ERR_LAUNCH;
+    configured[device] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(tiles * p.split, row_tiles, 1);
+  cfg.blockDim = dim3(kNumThreads, 1, 1);
+  cfg.dynamicSmemBytes = kRowsSmem;
+  cfg.stream = MB_STREAM(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, gated_dx_kernel, p, tw, td) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }

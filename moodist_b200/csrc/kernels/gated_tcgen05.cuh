@@ -531,5 +531,182 @@ __device__ __forceinline__ void gated_rows_body(const GatedParams& p, int width,
   }
 }
 
+// ---- input gradient of few rows --------------------------------------------------------------------------------------
+// dx[T, K] = dgu[T, 2F] w[2F, K], where 256 x 256 tiles would be too few to fill the GPU and each would walk all of 2F alone
+// (301 x 1016 over 5456: 8 tiles, 35 us; 17 us here). As above the weight is the M operand, here as it lies (MN-major): a CTA computes 128
+// columns of dx for up to 256 rows, and the `split` CTAs of a cluster share the steps over 2F and join their fp32 sums through
+// distributed shared memory, in rank order. Bound by the weight's bytes when T is small.
+enum DxStatus : uint32_t {
+  kTimeoutDxProducer = 0x141,
+  kTimeoutDxMma = 0x142,
+  kTimeoutDxEpilogue = 0x143,
+  kTimeoutDxDrain = 0x144,
+};
+struct DxParams {
+  int T, K, R;  // R = 2F, the length of the sums
+  __nv_bfloat16* dx;
+  int64_t lddx;
+  int n;      // rows per CTA, a multiple of 16 up to 256
+  int split;  // CTAs per cluster
+  uint32_t* status;
+  uint64_t wait_ns;
+};
+__host__ __device__ inline int dx_stage_bytes(int n) { return kATileBytes + n * 128; }
+__host__ __device__ inline int dx_stages(int n) {
+  const int fit = (kRowsSmem - 1024 - kRowsBars) / dx_stage_bytes(n);
+  return fit < kRowsMaxStages ? fit : kRowsMaxStages;
+}
+
+__device__ __forceinline__ void dx_report(const DxParams& p, uint32_t code) {
+  volatile uint32_t* s = p.status;
+  if (s && *s == 0) *s = code;
+}
+
+__device__ __forceinline__ void gated_dx_body(const DxParams& p, const CUtensorMap* tmap_w, const CUtensorMap* tmap_d, uint8_t* smem_raw) {
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* tiles = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const int n = p.n, split = p.split, stages = dx_stages(n), stage_bytes = dx_stage_bytes(n);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + stages * stage_bytes);  // [stages]
+  uint64_t* empty = full + kRowsMaxStages;                                     // [stages]
+  uint64_t* acc_full = empty + kRowsMaxStages;
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % split, col0 = blockIdx.x / split * BM, row0 = blockIdx.y * n;
+  const int all_steps = (p.R + BK - 1) / BK;
+  const int step0 = (int)((int64_t)all_steps * rank / split), steps = (int)((int64_t)all_steps * (rank + 1) / split) - step0;
+  const uint32_t tmem_cols = n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(tmap_w);
+    tma_prefetch_desc(tmap_d);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_base_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  body_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_base_slot;
+  grid_wait();
+  grid_release();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      bool ok = true;
+      int it = 0, s = 0;
+      uint32_t phase = 1;
+      uint8_t* sw = tiles;
+      for (; it < steps; ++it) {
+        if (!mbar_wait(&empty[s], phase, p.wait_ns)) {
+          dx_report(p, kTimeoutDxProducer);
+          ok = false;
+          break;
+        }
+        const int r0 = (step0 + it) * BK;
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+#pragma unroll
+        for (int c = 0; c < BM / 64; ++c) tma_load_2d(sw + c * 8192, tmap_w, &full[s], col0 + c * 64, r0);
+        tma_load_2d(sw + kATileBytes, tmap_d, &full[s], r0, row0);
+        sw += stage_bytes;
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1;
+          sw = tiles;
+        }
+      }
+      if (!ok) {
+        // let the copies still in flight land before this CTA's shared memory is given up
+        for (int i = it > stages ? it - stages : 0; i < it; ++i)
+          if (!mbar_wait(&full[i % stages], (i / stages) & 1, p.wait_ns)) dx_report(p, kTimeoutDxDrain);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc_f16(true, true, false, BM, n);
+      const uint64_t first_w = make_smem_desc(smem_u32(tiles), 8192, 1024);
+      const uint64_t first_d = make_smem_desc(smem_u32(tiles) + kATileBytes, 0, 1024);
+      bool ok = true;
+      int s = 0;
+      uint32_t phase = 0;
+      uint64_t dw = first_w, dd = first_d;
+      for (int it = 0; it < steps; ++it) {
+        if (!mbar_wait(&full[s], phase, p.wait_ns)) {
+          dx_report(p, kTimeoutDxMma);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k) tc_mma_f16(tmem_base, dw + k * (2048 >> 4), dd + k * 2, idesc, it | k);
+        tc_commit(&empty[s]);
+        dw += stage_bytes >> 4;
+        dd += stage_bytes >> 4;
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1;
+          dw = first_w;
+          dd = first_d;
+        }
+      }
+      if (ok) tc_commit(acc_full);
+    }
+  } else {
+    // accumulators to shared memory as sums[row][128 columns]: every product is done, so the stages are free
+    const int q = warp & 3, r = q * 32 + lane;
+    float* sums = reinterpret_cast<float*>(tiles);
+    if (mbar_wait(acc_full, 0, p.wait_ns)) {
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; c < n && row0 + c < p.T; c += 16) {
+        uint32_t v[16];
+        tmem_ld_32x16(taddr + c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(c + i) * BM + r] = __uint_as_float(v[i]);
+      }
+    } else if (lane == 0) {
+      dx_report(p, kTimeoutDxEpilogue);
+    }
+    tc_fence_before_sync();
+  }
+  body_sync();
+  if (split > 1) cluster_sync_all();  // every CTA of the cluster has its sums in place
+  {
+    const int rows = min(n, p.T - row0), pieces = rows * (BM / 8);
+    const uint32_t here = smem_u32(tiles);
+    for (int i = rank * kNumThreads + (int)threadIdx.x; i < pieces; i += split * kNumThreads) {
+      const int t = i / (BM / 8), j = i % (BM / 8) * 8, col = col0 + j;
+      if (col >= p.K) continue;
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = 0.f;
+      for (int c = 0; c < split; ++c) {
+        const uint32_t from = (split > 1 ? map_to_cta(here, c) : here) + (t * BM + j) * 4;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float4 a = ld_cluster_f4(from + k * 16);
+          f[4 * k] += a.x, f[4 * k + 1] += a.y, f[4 * k + 2] += a.z, f[4 * k + 3] += a.w;
+        }
+      }
+      store_vec<__nv_bfloat16, 8>(p.dx + (row0 + t) * p.lddx + col, f);
+    }
+  }
+  if (split > 1) cluster_sync_all();  // the peers no longer read this CTA's sums
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, tmem_cols);
+  }
+}
+
 }  // namespace gated
 }  // namespace mb

@@ -274,6 +274,9 @@ int mb_scale_by(void* x, int64_t n, int dtype, const float* s, void* stream);
 int mb_gated_scale_pitch(int F);
 int mb_gated_fwd_bf16(const void* x, const void* w, void* h, void* gu, void* scales, int64_t T, int F, int K, int64_t ldx, int64_t ldw,
                       int64_t ldh, int act, uint32_t* status, uint64_t wait_ns, void* stream);
+// dx[T, K] = dgu[T, 2F] w[2F, K].
+int mb_gated_dx_bf16(const void* dgu, const void* w, void* dx, int64_t T, int F, int K, int64_t lddgu, int64_t ldw, int64_t lddx,
+                     uint32_t* status, uint64_t wait_ns, void* stream);
 int mb_gated_bwd_bf16(const void* gu, const void* scales, const void* dh, void* dgu, int64_t T, int F, int64_t lddh, int act, void* stream);
 
 #ifdef __cplusplus
