@@ -1,7 +1,7 @@
 // Tensor-level entry points of the decoder operators (layer normalisation, rotary positions, distillation loss, gated
-// projection): checks of
-// arguments, autograd and the launches on the current stream of the tensors' device. The *_check functions are the same
-// checks for CPU tensors, whose arithmetic is in Python.
+// projection): checks of arguments, autograd and the launches on the current stream of the tensors' device. The *_check
+// functions are the same checks for CPU tensors, whose arithmetic is in Python.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -46,9 +46,22 @@ bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad() &
 
 at::Tensor value(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 
-// The kernels' backward passes give no graph of their own.
-void once(const char* what) {
+// What every backward pass asks for. The kernels' backward passes give no graph of their own. And one that is being captured
+// must not hand its gradients to a node of the default stream, which cannot join a capture: a leaf keeps its node as long as
+// any graph that used it lives, an eager one included, and an engine that finds the wait impossible ends the process.
+void backward_check(const char* what, const at::Device& device) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "moodist ", what, ": differentiable once (no create_graph)");
+  const auto stream = c10::cuda::getCurrentCUDAStream(device.index()), plain = c10::cuda::getDefaultCUDAStream(device.index());
+  const auto node = stream == plain ? nullptr : torch::autograd::get_current_node();
+  if (!node) return;
+  bool plain_receiver = false;
+  for (const auto& edge : node->next_edges())
+    if (edge.function) plain_receiver |= edge.function->stream() == std::optional<c10::Stream>(plain.unwrap());
+  if (!plain_receiver) return;
+  c10::cuda::CUDAGuard guard(device);
+  TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None, "moodist ", what,
+              ": the gradient of a captured backward pass would go to the default stream. An earlier graph of the same tensors, made "
+              "there, is still alive: release its outputs before the capture, or make it on another stream");
 }
 
 const void* ptr(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -113,9 +126,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("layer_norm");
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x2 = saved[0], &w = saved[1], &stats = saved[2];
+    backward_check("layer_norm", x2.device());
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     c10::cuda::CUDAGuard guard(x2.device());
     const int64_t rows = x2.size(0), D = x2.size(1), wants = ctx->saved_data["wants"].toInt();
@@ -152,6 +165,8 @@ void rotary_check(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos
   TORCH_CHECK(dtype_code(q.scalar_type()) >= 0, "moodist rotary: q must be bf16, fp16 or fp32, not ", q.scalar_type());
   TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "moodist rotary: q must be [batch, tokens, heads, dim] or [tokens, heads, dim], got ",
               q.sizes());
+  TORCH_CHECK(q.size(-1) <= (1 << 20) && q.size(-2) <= (1 << 20) && (!k.has_value() || k->dim() < 2 || k->size(-2) <= (1 << 20)),
+              "moodist rotary: at most 2^20 heads of 2^20 dimensions");
   if (k.has_value()) {
     TORCH_CHECK(k->dim() == q.dim() && k->size(-1) == q.size(-1) && k->sizes().slice(0, q.dim() - 2) == q.sizes().slice(0, q.dim() - 2),
                 "moodist rotary: k must have q's batch, tokens and head dimension, got ", k->sizes(), " for ", q.sizes());
@@ -236,8 +251,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("rotary");
     const auto saved = ctx->get_saved_variables();
+    backward_check("rotary", saved[0].device());
     at::Tensor gq = dense_last(grads[0]), gk = grads.size() > 1 ? dense_last(grads[1]) : at::Tensor();
     at::Tensor dq, dk;
     if (gq.defined()) dq = at::empty(gq.sizes(), gq.options());
@@ -384,9 +399,9 @@ struct Distill : torch::autograd::Function<Distill> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("distill_loss");
     variable_list out(9);
     if (!grads[0].defined()) return out;
+    backward_check("distill_loss", grads[0].device());
     auto& a = ctx->saved_data;
     at::Tensor g = grads[0].contiguous();
     if (a.count("grad")) {
@@ -437,7 +452,8 @@ void gated_check(const at::Tensor& x, const at::Tensor& w, const std::string& ac
               "moodist gated_linear: the weight must be [2 * features, ", x.dim() ? x.size(-1) : 0, "], gate rows first, got ", w.sizes());
   TORCH_CHECK(w.size(0) % 16 == 0 && w.size(1) % 8 == 0 && w.size(1) > 0,
               "moodist gated_linear: features and inputs must be multiples of 8, got a weight of ", w.sizes());
-  TORCH_CHECK(w.numel() < (1ll << 40) && x.numel() / x.size(-1) <= (1 << 30), "moodist gated_linear: too many rows");
+  TORCH_CHECK(w.numel() < (1ll << 40) && w.size(0) <= (1 << 30) && w.size(1) <= (1 << 30) && x.numel() / x.size(-1) <= (1 << 30),
+              "moodist gated_linear: at most 2^30 rows, inputs and rows of weight, got ", x.sizes(), " and ", w.sizes());
   TORCH_CHECK(x.device() == w.device(), "moodist gated_linear: tensors on one device required");
 }
 
@@ -483,8 +499,8 @@ struct Gated : torch::autograd::Function<Gated> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("gated_linear");
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+    backward_check("gated_linear", grads[0].device());
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x2 = saved[0], &w2 = saved[1], &gu = saved[2], &scales = saved[3];
     c10::cuda::CUDAGuard guard(x2.device());

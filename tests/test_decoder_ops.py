@@ -190,3 +190,15 @@ def test_refusals():
                 dict(x=x[:, :4]), dict(x=torch.randn(2, 6).bfloat16(), w=torch.randn(16, 6).bfloat16()), dict(x=torch.randn(2, 0).bfloat16(), w=w[:, :0])):
         with refused:
             gated_linear(**{"x": x, "w": w, **bad})
+
+
+def test_sizes_beyond_the_kernels_counters_are_refused():
+    wide = torch.zeros(1, 8).bfloat16()
+    with pytest.raises(RuntimeError, match="moodist gated_linear"):
+        gated_linear(wide, wide.expand(2**31, 8))
+    cos, sin = rotary_tables(2, 1)
+    for shape in ((1, 1, 2**20 + 1, 2), (1, 1, 1, 2**20 + 2)):
+        with pytest.raises(RuntimeError, match="moodist rotary"):
+            rotary(torch.zeros(1, 1, 1, 1).expand(shape), None, cos, sin)
+    with pytest.raises(RuntimeError, match="moodist rotary"):
+        rotary(torch.zeros(1, 1, 1, 2), torch.zeros(1, 1, 1, 2).expand(1, 1, 2**20 + 1, 2), cos, sin)

@@ -503,6 +503,53 @@ def test_decoder_block_captured_and_replayed():
                 assert (got.double() - value.double()).norm() <= 2.0**-7 * value.double().norm()  # attention's library backward may reorder
 
 
+def test_capture_beside_an_eager_graph_of_the_same_leaves():
+    """A captured backward pass whose leaves an eager graph of the default stream still holds cannot be joined: it is refused
+    by each operator, and runs once that graph is gone. One of another stream may live on."""
+    from moodist_b200.ops.gemm import gated_linear
+    from moodist_b200.ops.train import distill_loss, layer_norm, rotary, rotary_tables
+
+    cos, sin = rotary_tables(32, 16, device="cuda")
+    ids, top = torch.randint(0, 64, (16, 4), device="cuda"), _randn(16, 4)
+    x = _randn(16, 64, dtype=torch.bfloat16).requires_grad_()
+    w = _randn(64, 64, dtype=torch.bfloat16).requires_grad_()
+    calls = (lambda: layer_norm(x), lambda: rotary(x.view(16, 2, 32), None, cos, sin)[0], lambda: distill_loss(x, ids, top),
+             lambda: distill_loss(x.half(), ids, top), lambda: gated_linear(x, w))
+
+    def captured(call):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = torch.autograd.grad(call().float().sum(), x)[0]
+        return graph, out
+
+    for call in (calls[0], calls[2], calls[4]):  # x is the operator's own leaf
+        kept = call()
+        want = torch.autograd.grad(call().float().sum(), x)[0]
+        with pytest.raises(RuntimeError, match="default stream"):
+            captured(call)
+        del kept
+        graph, out = captured(call)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    side = torch.cuda.Stream()
+    for call in calls:
+        want = torch.autograd.grad(call().float().sum(), x)[0]
+        torch.cuda.synchronize()
+        graph, out = captured(call)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        with torch.cuda.stream(side):
+            kept = call()
+        torch.cuda.synchronize()
+        graph, out = captured(call)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del kept
+
+
 def test_operators_on_a_side_stream():
     """Each operator runs on the stream that is current, in order with what was queued there before."""
     from moodist_b200.ops.gemm import gated_linear
